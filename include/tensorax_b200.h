@@ -39,7 +39,8 @@ enum {
                               stage: 1 misaligned shared memory, 2/3/4 forward producer / MMA / softmax warp,
                               12/13/14 linear-kernel producer / MMA / split warps, 22/23/24 backward
                               producer / MMA / row warps, 32/34 decoding-kernel producer / row warps,
-                              42/43/44 layer-GEMM producer / MMA / summing warps */
+                              42/43/44 layer-GEMM producer / MMA / summing warps; 51 is a page or a row that a K/V cache
+                              call names and that does not exist */
     TX_ERR_UNSUPPORTED = 5
 };
 
@@ -303,6 +304,84 @@ typedef struct tx_sdpa_bwd_desc {
     void *stream;
 } tx_sdpa_bwd_desc;
 TX_API int tx_sdpa_backward(const tx_sdpa_bwd_desc *desc);
+
+/* ---- K/V cache in pages of 8-bit codes (no reference counterpart: tensorax has no cache; a serving loop that keeps K and V
+ *      as plain tensors uses tx_sdpa_forward with kv_lens).  A row -- one token of one K/V head -- is d codes that share an
+ *      fp32 scale:
+ *        TX_KV_E4M3  scale = 2^e, the smallest e with max|x| <= 448 * 2^e (e >= -126); code = x / scale rounded to e4m3
+ *        TX_KV_INT8  scale = max|x| / 127 (2^-126 at least); code = x / scale rounded to the nearest integer, ties to even
+ *      and stands for code * scale.  A row with an infinity or a NaN gets the scale NaN and zero codes: it reads back as NaN,
+ *      and attention gives NaN to the rows that see it and to no others.
+ *      Token `pos` of sequence b lies in page page_table[b][pos / page_size], place pos % page_size.  Pages may be shared
+ *      between sequences as long as nobody writes them; two rows of one call that are written to one place race.
+ *      All pointers are device pointers (k, v, q, out and the codes 16-byte aligned), everything is asynchronous on `stream`
+ *      and captures into graphs; no call allocates.  A token without a page (a position beyond the table, an entry outside
+ *      [0, pages)) is left out, never followed, and reported: tx_sdpa_finish then returns TX_ERR_KERNEL (stage code 51), and
+ *      attention rows of the sequences concerned are NaN. */
+enum { TX_KV_E4M3 = 0, TX_KV_INT8 = 1 };
+typedef struct tx_kv_cache {
+    void *k, *v;              /* [pages, kv_heads, page_size, d] codes, a byte each */
+    float *k_scale, *v_scale; /* [pages, kv_heads, page_size] */
+    int64_t pages, kv_heads;
+    int64_t page_size;        /* a power of two, 16 at least */
+    int64_t d;                /* 64, 128 or 256 (of K and of V) */
+    int32_t format;           /* TX_KV_* */
+    int32_t reserved;
+} tx_kv_cache;
+
+/* Quantise the call's keys and values into the cache: token t of sequence b goes to position start[b] + t. */
+typedef struct tx_kv_write_desc {
+    tx_kv_cache cache;
+    const void *k, *v;           /* [batch, kv_heads, src_tokens, d] dtype */
+    const int32_t *page_table;   /* [batch, table_len] */
+    const int32_t *start;        /* optional [batch]: position of token 0 (NULL: 0) */
+    const int32_t *counts;       /* optional [batch]: tokens t >= counts[b] are not written (NULL: all are) */
+    const int32_t *rows;         /* optional [batch, tokens]: token t is row rows[b][t] of k and v (NULL: row t) -- the
+                                    accepted nodes of a tree of drafted tokens, brought into line */
+    int64_t batch, tokens, table_len;
+    int64_t src_tokens;          /* rows a head of k and v has; 0: `tokens` */
+    int32_t dtype;               /* TX_DTYPE_* of k and v */
+    int32_t flags;               /* 0 */
+    void *stream;
+} tx_kv_write_desc;
+TX_API int tx_kv_cache_write(const tx_kv_write_desc *desc);
+
+/* The values that tokens start[b] .. start[b] + counts[b] - 1 stand for, to rows 0 .. counts[b] - 1 of k and v (the product
+ * code * scale in fp32, rounded once to dtype).  Rows behind them are left as they were. */
+typedef struct tx_kv_read_desc {
+    tx_kv_cache cache;
+    void *k, *v;                 /* [batch, kv_heads, tokens, d] dtype */
+    const int32_t *page_table;   /* [batch, table_len] */
+    const int32_t *start;        /* optional [batch] (NULL: 0) */
+    const int32_t *counts;       /* optional [batch] (NULL: tokens) */
+    int64_t batch, tokens, table_len;
+    int32_t dtype;
+    int32_t flags;               /* 0 */
+    void *stream;
+} tx_kv_read_desc;
+TX_API int tx_kv_cache_read(const tx_kv_read_desc *desc);
+
+/* Attention of the last tokens of each sequence -- one decoding step, a chain, or a tree of drafted tokens -- over the cache,
+ * into which they have been written.  Sequence b has kv_lens[b] keys of which the last n = q_lens[b] are this call's nodes;
+ * ctx = kv_lens[b] - n.  Node t sees key j < ctx (with a window: where j > ctx + depth(t) - window or j < sinks; depth(t) is
+ * the number of nodes it sees beside itself) and node u iff bit u of tree[b][t] is set (without `tree`: iff u <= t).  A row that
+ * sees nothing is NaN.  Rows of nodes t >= n are left as they were.  fp16 queries: fp16 products, fp32 sums; fp32 queries:
+ * fp32-grade products of the codes' values. */
+typedef struct tx_kv_attention_desc {
+    tx_kv_cache cache;
+    const void *q;               /* [batch, q_heads, tokens, d] dtype */
+    void *out;                   /* the same, fp32 (fp16 with TX_SDPA_OUT_F16) */
+    const int32_t *page_table;   /* [batch, table_len] */
+    const int32_t *kv_lens;      /* [batch] */
+    const int32_t *q_lens;       /* optional [batch] (NULL: tokens) */
+    const uint64_t *tree;        /* optional [batch, tokens]; bits of nodes that a sequence does not have are clear */
+    int64_t batch, q_heads, tokens, table_len;   /* tokens: 1 to 64; q_heads a multiple of cache.kv_heads */
+    int64_t window, sinks;       /* window 0: none; else at least `tokens` */
+    int32_t dtype;               /* TX_DTYPE_* of q */
+    int32_t flags;               /* TX_SDPA_OUT_F16 */
+    void *stream;
+} tx_kv_attention_desc;
+TX_API int tx_kv_cache_attention(const tx_kv_attention_desc *desc);
 
 /* ---- host-buffer form (no reference counterpart): `desc` holds HOST pointers
  *      (q, k, v, kv_lens, out; mask must be NULL).  Copies in, runs, copies out,

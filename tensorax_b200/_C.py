@@ -452,3 +452,165 @@ def scaled_dot_product_attention_ex(query, key, value, mask=None, causal=False, 
         flags = int(flags) | _lib.TX_SDPA_F32_VIA_F16
     return _forward(query, key, value, mask, causal=causal, kv_lens=kv_lens, flags=flags, out_dtype=out_dtype,
                     want_lse=want_lse, sync=sync)
+
+
+# ------------------------------------------------------------------ quantised K/V cache (no reference counterpart)
+class IndexImpl:
+    """Whole numbers on the device (page tables, lengths, positions, row lists: int32; a tree's words: uint64).  A serving
+    loop builds them once and passes them to every call; the calls also take plain lists and arrays, and upload those."""
+
+    __slots__ = ("shape", "dtype", "_buf")
+
+    def __init__(self, array, dtype=np.int32):
+        a = np.asarray(array)
+        info = np.iinfo(dtype)
+        if a.dtype.kind not in "iu" or (a.size and (int(a.min()) < info.min or int(a.max()) > info.max)):
+            raise RuntimeError(f"index array: whole numbers that {np.dtype(dtype).name} holds expected")
+        self.shape, self.dtype = tuple(a.shape), np.dtype(dtype)
+        self._buf = _lib.to_device(a.astype(dtype))
+
+    data_ptr = property(lambda self: self._buf.ptr)
+
+
+def index_array(x, shape, who, name, dtype=np.int32):
+    """`x` (None stays None) on the device, its shape checked."""
+    if x is None:
+        return None
+    have = tuple(x.shape) if isinstance(x, IndexImpl) else np.shape(x)
+    if have != tuple(shape):
+        raise RuntimeError(f"{who}: {name} must have shape {list(shape)}")
+    if not isinstance(x, IndexImpl):
+        return IndexImpl(x, dtype)
+    if x.dtype != np.dtype(dtype):
+        raise RuntimeError(f"{who}: {name} must hold {np.dtype(dtype).name}")
+    return x
+
+
+_KV_FORMATS = {"e4m3": _lib.TX_KV_E4M3, "int8": _lib.TX_KV_INT8}
+
+
+class KvCacheImpl:
+    """Device memory of a K/V cache: codes [pages, kv_heads, page_size, d] and scales [pages, kv_heads, page_size] of K and V."""
+
+    __slots__ = ("pages", "kv_heads", "page_size", "d", "format", "_bufs")
+
+    def __init__(self, pages, kv_heads, page_size, d, format):
+        if format not in _KV_FORMATS:
+            raise RuntimeError("K/V cache: format must be 'e4m3' or 'int8'")
+        if min(pages, kv_heads) <= 0 or d not in (64, 128, 256):
+            raise RuntimeError("K/V cache: pages and kv_heads must be positive, the head dim 64, 128 or 256")
+        if not 16 <= page_size <= 65536 or page_size & (page_size - 1):
+            raise RuntimeError("K/V cache: page_size must be a power of two from 16 to 65536")
+        self.pages, self.kv_heads, self.page_size, self.d, self.format = int(pages), int(kv_heads), int(page_size), int(d), format
+        rows = self.pages * self.kv_heads * self.page_size
+        self._bufs = [_lib.DeviceBuffer(rows * d), _lib.DeviceBuffer(rows * d), _lib.DeviceBuffer(rows * 4), _lib.DeviceBuffer(rows * 4)]
+
+    @property
+    def desc(self):
+        k, v, ks, vs = (b.ptr for b in self._bufs)
+        return _lib.KvCache(k=k, v=v, k_scale=ks, v_scale=vs, pages=self.pages, kv_heads=self.kv_heads, page_size=self.page_size,
+                            d=self.d, format=_KV_FORMATS[self.format])
+
+    def to_numpy(self):
+        """Codes (uint8 for e4m3, int8 for int8) and scales of K and of V."""
+        shape = (self.pages, self.kv_heads, self.page_size)
+        codes = np.uint8 if self.format == "e4m3" else np.int8
+        return ([self._bufs[i].download((*shape, self.d), codes) for i in (0, 1)],
+                [self._bufs[i].download(shape, np.float32) for i in (2, 3)])
+
+
+def _kv_ptr(x):
+    return x.data_ptr if x is not None else None
+
+
+def _kv_table(cache, page_table, batch, who):
+    shape = tuple(page_table.shape) if isinstance(page_table, IndexImpl) else np.shape(page_table)
+    if len(shape) != 2 or shape[0] != batch:
+        raise RuntimeError(f"{who}: page_table must be [batch, pages of a sequence]")
+    return index_array(page_table, shape, who, "page_table"), shape[1]
+
+
+def _kv_dtype(t, who):
+    if t.device != "cuda":
+        raise RuntimeError(f"{who}: tensorax_b200 implements the CUDA path only")
+    return _lib.TX_DTYPE_F16 if t.dtype in ("float16", "half") else _lib.TX_DTYPE_F32
+
+
+def kv_cache_write(cache, key, value, page_table, start=None, counts=None, rows=None, sync=True) -> None:
+    """Quantise key and value [B, kv_heads, T, d] into the cache's pages: token t of sequence b goes to position start[b] + t
+    of its page table; tokens from counts[b] on are left out.  `rows` [B, n]: n tokens are written instead, of which token t
+    is row rows[b][t] of key and value."""
+    who = "K/V cache write"
+    if len(key._shape) != 4 or key._shape != value._shape or key.dtype != value.dtype or key.device != value.device:
+        raise RuntimeError(f"{who}: key and value must be 4D tensors of one shape, dtype and device")
+    B, H, T, d = key._shape
+    if H != cache.kv_heads or d != cache.d:
+        raise RuntimeError(f"{who}: key and value must be [batch, kv_heads, tokens, d] of the cache")
+    dtype = _kv_dtype(key, who)
+    table, table_len = _kv_table(cache, page_table, B, who)
+    n = T
+    if rows is not None:
+        n = (rows.shape if isinstance(rows, IndexImpl) else np.shape(rows))[-1]
+        rows = index_array(rows, (B, n), who, "rows")
+    start, counts = index_array(start, (B,), who, "start"), index_array(counts, (B,), who, "counts")
+    lib = _lib.load()
+    desc = _lib.KvWriteDesc(cache=cache.desc, k=key.data_ptr, v=value.data_ptr, page_table=_kv_ptr(table), start=_kv_ptr(start),
+                            counts=_kv_ptr(counts), rows=_kv_ptr(rows), batch=B, tokens=n, table_len=table_len, src_tokens=T,
+                            dtype=dtype, flags=0, stream=None)
+    _lib.check(lib.tx_kv_cache_write(ctypes.byref(desc)))
+    if sync:
+        _lib.check(lib.tx_sdpa_finish(None))
+
+
+def kv_cache_read(cache, page_table, tokens, start=None, counts=None, dtype="float16", sync=True):
+    """The values of `tokens` tokens from start[b] on, (K, V) [B, kv_heads, tokens, d]; rows from counts[b] on are zero."""
+    who = "K/V cache read"
+    B = (page_table.shape if isinstance(page_table, IndexImpl) else np.shape(page_table))[0]
+    table, table_len = _kv_table(cache, page_table, B, who)
+    start, counts_dev = index_array(start, (B,), who, "start"), index_array(counts, (B,), who, "counts")
+    if dtype not in ("float16", "float32"):
+        raise RuntimeError(f"{who}: dtype must be 'float32' or 'float16'")
+    shape = [B, cache.kv_heads, int(tokens), cache.d]
+    if counts is None:
+        out = [TensorImpl(shape, dtype, "cuda") for _ in range(2)]
+    else:                                            # the library leaves rows behind a sequence's count as they were
+        out = [from_numpy(np.zeros(shape, _NP[dtype])) for _ in range(2)]
+    lib = _lib.load()
+    desc = _lib.KvReadDesc(cache=cache.desc, k=out[0].data_ptr, v=out[1].data_ptr, page_table=_kv_ptr(table),
+                           start=_kv_ptr(start), counts=_kv_ptr(counts_dev), batch=B, tokens=int(tokens), table_len=table_len,
+                           dtype=_lib.TX_DTYPE_F16 if dtype == "float16" else _lib.TX_DTYPE_F32, flags=0, stream=None)
+    _lib.check(lib.tx_kv_cache_read(ctypes.byref(desc)))
+    if sync:
+        _lib.check(lib.tx_sdpa_finish(None))
+    return out
+
+
+def kv_cache_attention(cache, query, page_table, kv_lens, q_lens=None, tree=None, window=None, sinks=0, out_dtype="float32",
+                       sync=True) -> TensorImpl:
+    """Attention of the last tokens of each sequence over the cache: query [B, Hq, T, d], T <= 64, kv_lens [B] keys of each
+    sequence, the last q_lens[b] (T) of them this call's.  `tree` [B, T]: bit u of a node's word says that it sees node u."""
+    who = "K/V cache attention"
+    if len(query._shape) != 4 or query._shape[3] != cache.d or query._shape[1] % cache.kv_heads:
+        raise RuntimeError(f"{who}: query must be [batch, heads, tokens, d], heads a multiple of the cache's")
+    if out_dtype not in ("float32", "float16"):
+        raise RuntimeError(f"{who}: out_dtype must be 'float32' or 'float16'")
+    B, Hq, T, d = query._shape
+    dtype = _kv_dtype(query, who)
+    table, table_len = _kv_table(cache, page_table, B, who)
+    kv_lens_dev, q_lens_dev = index_array(kv_lens, (B,), who, "kv_lens"), index_array(q_lens, (B,), who, "q_lens")
+    tree = index_array(tree, (B, T), who, "tree", np.uint64)
+    if kv_lens_dev is None:
+        raise RuntimeError(f"{who}: kv_lens must hold one length per batch element")
+    if q_lens is None:
+        out = TensorImpl(query._shape, out_dtype, "cuda")
+    else:                                            # rows of nodes that a sequence does not have are left as they were
+        out = from_numpy(np.zeros(query._shape, _NP[out_dtype]))
+    lib = _lib.load()
+    desc = _lib.KvAttentionDesc(cache=cache.desc, q=query.data_ptr, out=out.data_ptr, page_table=_kv_ptr(table),
+                                kv_lens=_kv_ptr(kv_lens_dev), q_lens=_kv_ptr(q_lens_dev), tree=_kv_ptr(tree), batch=B, q_heads=Hq,
+                                tokens=T, table_len=table_len, window=0 if window is None else int(window), sinks=int(sinks),
+                                dtype=dtype, flags=_lib.TX_SDPA_OUT_F16 if out_dtype == "float16" else 0, stream=None)
+    _lib.check(lib.tx_kv_cache_attention(ctypes.byref(desc)))
+    if sync:
+        _lib.check(lib.tx_sdpa_finish(None))
+    return out

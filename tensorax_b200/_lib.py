@@ -22,6 +22,8 @@ TX_SDPA_OUT_F16 = 4
 TX_SDPA_F32_VIA_F16 = 8
 TX_SDPA_KV_LENS_HOST = 16
 TX_MHA_F16_ATTENTION = 32
+TX_KV_E4M3 = 0
+TX_KV_INT8 = 1
 TX_ERR_UNSUPPORTED = 5
 
 # every symbol include/tensorax_b200.h declares
@@ -40,6 +42,7 @@ EXPORTED_SYMBOLS = (
     "tx_sdpa_mma_profile_sections_cuda", "tx_sdpa_optimized_flash_profile_sections_cuda",
     "tx_selftest_wait_timeout", "tx_sdpa_forward_host_copies_only", "tx_sdpa_set_group_l2_bytes",
     "tx_mha_forward_f32",
+    "tx_kv_cache_write", "tx_kv_cache_read", "tx_kv_cache_attention",
 )
 
 
@@ -75,6 +78,46 @@ class MhaDesc(ctypes.Structure):
         ("mask", c_void_p), ("kv_lens", c_void_p), ("out", c_void_p),
         ("batch", c_int64), ("seq_q", c_int64), ("seq_k", c_int64), ("embed", c_int64), ("heads", c_int64),
         ("causal", c_int32), ("flags", c_int32), ("stream", c_void_p),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of ``tx_kv_cache``."""
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("pages", c_int64), ("kv_heads", c_int64), ("page_size", c_int64), ("d", c_int64),
+        ("format", c_int32), ("reserved", c_int32),
+    ]
+
+
+class KvWriteDesc(ctypes.Structure):
+    """Mirror of ``tx_kv_write_desc``."""
+    _fields_ = [
+        ("cache", KvCache), ("k", c_void_p), ("v", c_void_p), ("page_table", c_void_p), ("start", c_void_p),
+        ("counts", c_void_p), ("rows", c_void_p),
+        ("batch", c_int64), ("tokens", c_int64), ("table_len", c_int64), ("src_tokens", c_int64),
+        ("dtype", c_int32), ("flags", c_int32), ("stream", c_void_p),
+    ]
+
+
+class KvReadDesc(ctypes.Structure):
+    """Mirror of ``tx_kv_read_desc``."""
+    _fields_ = [
+        ("cache", KvCache), ("k", c_void_p), ("v", c_void_p), ("page_table", c_void_p), ("start", c_void_p),
+        ("counts", c_void_p),
+        ("batch", c_int64), ("tokens", c_int64), ("table_len", c_int64),
+        ("dtype", c_int32), ("flags", c_int32), ("stream", c_void_p),
+    ]
+
+
+class KvAttentionDesc(ctypes.Structure):
+    """Mirror of ``tx_kv_attention_desc``."""
+    _fields_ = [
+        ("cache", KvCache), ("q", c_void_p), ("out", c_void_p), ("page_table", c_void_p), ("kv_lens", c_void_p),
+        ("q_lens", c_void_p), ("tree", c_void_p),
+        ("batch", c_int64), ("q_heads", c_int64), ("tokens", c_int64), ("table_len", c_int64),
+        ("window", c_int64), ("sinks", c_int64),
+        ("dtype", c_int32), ("flags", c_int32), ("stream", c_void_p),
     ]
 
 
@@ -132,6 +175,9 @@ def load():
     lib.tx_sdpa_finish.argtypes = [c_void_p]
     lib.tx_sdpa_fp16_static_scratch.argtypes = [c_void_p] * 4 + [c_int64] * 6 + [c_int32, c_void_p, c_void_p]
     lib.tx_mha_forward_f32.argtypes = [ctypes.POINTER(MhaDesc)]
+    lib.tx_kv_cache_write.argtypes = [ctypes.POINTER(KvWriteDesc)]
+    lib.tx_kv_cache_read.argtypes = [ctypes.POINTER(KvReadDesc)]
+    lib.tx_kv_cache_attention.argtypes = [ctypes.POINTER(KvAttentionDesc)]
     lib.tx_kernel_launch_count.restype = c_int64
     _lib = lib
     return lib

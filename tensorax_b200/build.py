@@ -5,6 +5,7 @@ nvcc cross-compiles for sm_100a without a GPU.  The output,
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -13,12 +14,12 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(CSRC, "libtensorax_b200.so")
-SOURCES = ["sdpa_api.cu"]
-HEADERS = ["ptx.cuh", "kv_lens.cuh", "sdpa_simt.cuh", "sdpa_tc.cuh", "sdpa_tc_pair.cuh", "sdpa_tc_x3.cuh", "bounded_wait.h", "status_report.h", "sdpa_bwd.cuh", "sdpa_decode.cuh", "linear_simt.cuh", "linear_tc.cuh", "gemm_x3.cuh", os.path.join("..", "..", "include", "tensorax_b200.h")]
+SOURCES = ["sdpa_api.cu", "kv_cache_api.cu"]
+HEADERS = ["ptx.cuh", "kv_lens.cuh", "sdpa_simt.cuh", "sdpa_tc.cuh", "sdpa_tc_pair.cuh", "sdpa_tc_x3.cuh", "bounded_wait.h", "status_report.h", "sdpa_bwd.cuh", "sdpa_decode.cuh", "linear_simt.cuh", "linear_tc.cuh", "gemm_x3.cuh", "api_internal.h", "kv_cache.cuh", "kv_attention.cuh", os.path.join("..", "..", "include", "tensorax_b200.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--compiler-options", "-fPIC,-fvisibility=hidden", "-shared",
+    "--compiler-options", "-fPIC,-fvisibility=hidden",
 ]
 
 
@@ -38,15 +39,21 @@ def up_to_date() -> bool:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date():
         return OUT
-    cmd = [_nvcc(), *NVCC_FLAGS]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    cmd += ["-o", OUT, *[os.path.join(CSRC, s) for s in SOURCES]]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose:
-        sys.stderr.write(proc.stderr)
-    if proc.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + proc.stderr[-4000:])
+    def run(cmd):
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose:
+            sys.stderr.write(proc.stderr)
+        if proc.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + proc.stderr[-4000:])
+
+    more = ["-Xptxas", "-v"] if verbose else []
+    objects = [os.path.join(CSRC, os.path.splitext(s)[0] + ".o") for s in SOURCES]
+    with concurrent.futures.ThreadPoolExecutor() as pool:      # the translation units side by side
+        list(pool.map(lambda so: run([_nvcc(), *NVCC_FLAGS, *more, "-c", "-o", so[1], os.path.join(CSRC, so[0])]),
+                      zip(SOURCES, objects)))
+    run([_nvcc(), *NVCC_FLAGS, "-shared", "-o", OUT, *objects])
+    for o in objects:
+        os.remove(o)
     return OUT
 
 

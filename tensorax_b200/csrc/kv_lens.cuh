@@ -29,7 +29,7 @@ struct KvLensChunk {
     int32_t n, val[kMax];
 };
 
-__global__ void __launch_bounds__(256) put_kv_lens_kernel(const __grid_constant__ KvLensChunk c, int32_t *__restrict__ dst)
+static __global__ void __launch_bounds__(256) put_kv_lens_kernel(const __grid_constant__ KvLensChunk c, int32_t *__restrict__ dst)
 {
     for (int i = threadIdx.x; i < c.n; i += blockDim.x) dst[i] = c.val[i];
 }

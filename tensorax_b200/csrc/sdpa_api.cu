@@ -40,6 +40,7 @@
 #include "sdpa_simt.cuh"
 #include "sdpa_bwd.cuh"
 #include "sdpa_decode.cuh"
+#include "api_internal.h"
 
 namespace {
 
@@ -966,6 +967,9 @@ int finish(cudaStream_t st)
         [&](int v) { return __atomic_exchange_n(const_cast<int *>(g_status[dev].mirror), v, __ATOMIC_SEQ_CST); },
         // the word only: the mirror's address stays behind it
         [&] { return cudaMemset(g_status[dev].word, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess; });
+    if (code == txb::KV_ERR_PAGE)
+        return fail(TX_ERR_KERNEL, "K/V cache: a token lies outside its sequence's page table, or the table or the row list names "
+                                   "a page or row that does not exist (stage code %d); output is not valid", code);
     if (code != 0)
         return fail(TX_ERR_KERNEL, "SDPA kernel gave up on a bounded wait (stage code %d); output is not valid", code);
     return TX_OK;
@@ -1347,6 +1351,29 @@ int pool_ready()
 }
 
 }  // namespace
+
+// What the library's other translation units use of this one (api_internal.h)
+namespace txb {
+namespace api {
+
+int fail(int code, const char *fmt, ...)
+{
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_err = buf;
+    return code;
+}
+int ensure_device() { return ::ensure_device(); }
+int status_word(int **out) { return ::status_word(out); }
+int sm_count(int *n) { return ::sm_count(n); }
+int current_device(int *dev) { return ::current_device(dev); }
+void launched() { g_launches++; }
+
+}  // namespace api
+}  // namespace txb
 
 extern "C" {
 
@@ -1942,6 +1969,9 @@ int tx_sdpa_fp16_static_scratch(const void *Q_h, const void *K_h, const void *V_
     int code = 0;
     TX_CUDA(cudaMemcpyAsync(&code, status, sizeof code, cudaMemcpyDeviceToHost, st));
     TX_CUDA(cudaStreamSynchronize(st));
+    if (code == txb::KV_ERR_PAGE)
+        return fail(TX_ERR_KERNEL, "K/V cache: a token lies outside its sequence's page table, or the table or the row list names "
+                                   "a page or row that does not exist (stage code %d); output is not valid", code);
     if (code != 0)
         return fail(TX_ERR_KERNEL, "SDPA kernel gave up on a bounded wait (stage code %d); output is not valid", code);
     return TX_OK;

@@ -150,3 +150,42 @@ def scaled_dot_product_attention_ex(query: Tensor, key: Tensor, value: Tensor,
     if needs_grad:
         return _result(c, True, ("scaled_dot_product_attention", query, key, value, mask))
     return _result(c)
+
+
+# ------------------------------------------------------------------ quantised K/V cache (no reference counterpart)
+def _check_cache(cache, *tensors):
+    if not _C:
+        raise RuntimeError("C++ backend not available.")
+    if any(len(t.shape) != 4 for t in tensors):
+        raise ValueError("K/V cache: tensors must be 4D [batch, heads, tokens, d]")
+    if any(t.device != "cuda" for t in tensors):
+        raise ValueError("K/V cache: only CUDA tensors supported")
+
+
+def kv_cache_write(cache, key: Tensor, value: Tensor, page_table, start=None, counts=None, rows=None, sync: bool = True) -> None:
+    """Quantise ``key`` and ``value`` [B, kv_heads, T, d] into the pages of ``cache`` (``nn.QuantizedKVCache``): token t of
+    sequence b goes to position ``start[b] + t`` (``start`` None: t), tokens from ``counts[b]`` on are left out.  ``rows``
+    [B, n]: write n tokens, of which token t is row ``rows[b][t]`` -- the accepted nodes of a tree of drafted tokens."""
+    _check_cache(cache, key, value)
+    _C.kv_cache_write(cache._impl, key._c_tensor, value._c_tensor, page_table, start, counts, rows, sync)
+
+
+def kv_cache_read(cache, page_table, tokens: int, start=None, counts=None, dtype: str = "float16", sync: bool = True):
+    """What the cache holds of ``tokens`` tokens from position ``start[b]`` on, as values: (K, V) [B, kv_heads, tokens, d].
+    Rows from ``counts[b]`` on are zero."""
+    _check_cache(cache)
+    k, v = _C.kv_cache_read(cache._impl, page_table, tokens, start, counts, dtype, sync)
+    return _result(k), _result(v)
+
+
+def kv_cache_attention(query: Tensor, cache, page_table, kv_lens, q_lens=None, tree=None, window: Optional[int] = None,
+                       sinks: int = 0, out_dtype: str = "float32", sync: bool = True) -> Tensor:
+    """Attention of each sequence's last tokens over the cache they have been written to: one decoding step (T = 1), a chain, or
+    with ``tree`` a tree of drafted tokens.  ``query`` [B, heads, T, d] with T <= 64; ``kv_lens[b]`` keys of sequence b, of
+    which the last ``q_lens[b]`` (T) are this call's nodes; bit u of ``tree[b][t]`` says that node t sees node u (itself
+    included).  ``window``: a node sees only that many positions up to its own, and the first ``sinks`` keys.  No gradient."""
+    _check_cache(cache, query)
+    if query.requires_grad:
+        raise ValueError("K/V cache: attention over a cache has no backward pass")
+    return _result(_C.kv_cache_attention(cache._impl, query._c_tensor, page_table, kv_lens, q_lens, tree, window, sinks,
+                                         out_dtype, sync))

@@ -2,6 +2,7 @@
 from .attention import (  # noqa: F401
     GroupedQueryAttention,
     MultiHeadAttention,
+    QuantizedKVCache,
     ScaledDotProductAttention,
     create_causal_mask,
     create_padding_mask,

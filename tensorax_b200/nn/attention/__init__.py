@@ -1,3 +1,4 @@
+from .cache import QuantizedKVCache
 from .layers import GroupedQueryAttention, MultiHeadAttention, ScaledDotProductAttention
 from .utils import create_causal_mask, create_padding_mask
 
@@ -7,4 +8,5 @@ __all__ = [
     "MultiHeadAttention",
     "create_causal_mask",
     "create_padding_mask",
+    "QuantizedKVCache",
 ]
