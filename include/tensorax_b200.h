@@ -305,11 +305,31 @@ typedef struct tx_sdpa_bwd_desc {
 } tx_sdpa_bwd_desc;
 TX_API int tx_sdpa_backward(const tx_sdpa_bwd_desc *desc);
 
+/* ---- sliding window with sinks (no reference counterpart: the reference could only express it as a dense mask).  Row i of
+ *      sequence b stands at position p = i, or with align_end at len_b - seq_q + i: the rows are then the last ones of their
+ *      sequence, as in a decoding step or in a chunk of a long prompt (len_b: kv_lens[b], or seq_k).  It sees key j iff
+ *      j < len_b, j <= p, and (j > p - window or j < sinks).  Keys that no row of a tile sees are not read.
+ *      The forward descriptor is that of tx_sdpa_forward with `causal` nonzero and without a dense mask; flags
+ *      TX_SDPA_OUT_F16, TX_SDPA_KV_LENS_HOST, TX_SDPA_FORCE_SIMT.  All of its types and head dims, `lse` included.
+ *      A row that sees no key is NaN; rows from kv_lens[b] on of K and V may hold anything.  A value that is not finite at a
+ *      key that one row of a 128-row tile sees may show in the tile's other rows.
+ *      Backward: as tx_sdpa_backward (fp16, d in {64, 128, 256}); a row that sees no key has gradient zero and adds nothing to
+ *      those of K and V.  TX_BWD_GRADS_F16: dq, dk, dv are fp16. */
+enum { TX_BWD_GRADS_F16 = 64 };
+typedef struct tx_window_desc {
+    int64_t window;              /* 1 at least: a row's own position counts */
+    int64_t sinks;               /* first keys that stay visible; 0: none */
+    int32_t align_end;
+    int32_t reserved;
+} tx_window_desc;
+TX_API int tx_sdpa_window_forward(const tx_sdpa_desc *desc, const tx_window_desc *window);
+TX_API int tx_sdpa_window_backward(const tx_sdpa_bwd_desc *desc, const tx_window_desc *window);
+
 /* ---- K/V cache in pages of 8-bit codes (no reference counterpart: tensorax has no cache; a serving loop that keeps K and V
  *      as plain tensors uses tx_sdpa_forward with kv_lens).  A row -- one token of one K/V head -- is d codes that share an
  *      fp32 scale:
  *        TX_KV_E4M3  scale = 2^e, the smallest e with max|x| <= 448 * 2^e (e >= -126); code = x / scale rounded to e4m3
- *        TX_KV_INT8  scale = max|x| / 127 (2^-126 at least); code = x / scale rounded to the nearest integer, ties to even
+ *        TX_KV_INT8  scale = max|x| * (1/127) in fp32 (2^-126 at least); code = x / scale rounded to the nearest integer, ties to even
  *      and stands for code * scale.  A row with an infinity or a NaN gets the scale NaN and zero codes: it reads back as NaN,
  *      and attention gives NaN to the rows that see it and to no others.
  *      Token `pos` of sequence b lies in page page_table[b][pos / page_size], place pos % page_size.  Pages may be shared

@@ -272,7 +272,7 @@ def synchronize() -> None:
 
 
 def _forward(query, key, value, mask, causal=False, kv_lens=None, flags=0, who="SDPA", out_dtype="float32",
-             want_lse=False, sync=True):
+             want_lse=False, sync=True, window=None):
     B, H, Hkv, Sq, Sk, dk, dv = _validate(query, key, value, mask, who)
     if query.device != "cuda":
         raise RuntimeError(
@@ -303,7 +303,10 @@ def _forward(query, key, value, mask, causal=False, kv_lens=None, flags=0, who="
         dtype=_lib.TX_DTYPE_F16 if f16 else _lib.TX_DTYPE_F32, causal=int(bool(causal)),
         flags=int(flags), stream=None, lse=lse.data_ptr if lse is not None else None)
     lib = _lib.load()
-    _lib.check(lib.tx_sdpa_forward(ctypes.byref(desc)))
+    if window is None:
+        _lib.check(lib.tx_sdpa_forward(ctypes.byref(desc)))
+    else:
+        _lib.check(lib.tx_sdpa_window_forward(ctypes.byref(desc), ctypes.byref(window)))
     if sync:
         _lib.check(lib.tx_sdpa_finish(None))   # the reference launchers return a finished result
     # sync=False: the launch is stream-ordered and has taken the key lengths with it
@@ -317,12 +320,14 @@ def sdpa_backward_supported(query, key, value, mask) -> bool:
             and query._shape[3] == value._shape[3] and query._shape[3] in (64, 128, 256))
 
 
-def scaled_dot_product_attention_backward(query, key, value, out, lse, grad, causal=False, kv_lens=None):
+def scaled_dot_product_attention_backward(query, key, value, out, lse, grad, causal=False, kv_lens=None, window=None,
+                                          grad_dtype="float32"):
     """Gradients (dq, dk, dv), float32, of ``out = SDPA(query, key, value)`` for the upstream
     gradient ``grad`` -- the reference's autograd rule, tensorax/tensor.py:806-827, which there
     runs through dense [Sq,Sk] temporaries (and cannot run at all: Tensor.transpose rejects the
     negative dims it is called with, tensorax/tensor.py:963-964).  ``lse`` is the row statistic
-    the forward returned with ``want_lse``."""
+    the forward returned with ``want_lse``.  ``window`` (a ``_lib.WindowDesc``): the forward was
+    ``scaled_dot_product_attention_window``'s; its gradients may be float16 (``grad_dtype``)."""
     B, H, Hkv, Sq, Sk, dk, dv = _validate(query, key, value, None, "SDPA backward")
     if not sdpa_backward_supported(query, key, value, None):
         raise RuntimeError("SDPA backward: built for float16 CUDA tensors with d_k == d_v in {64, 128, 256} and "
@@ -331,10 +336,14 @@ def scaled_dot_product_attention_backward(query, key, value, out, lse, grad, cau
         raise RuntimeError("SDPA backward: grad must be a float32 CUDA tensor shaped like the output")
     if list(out._shape) != [B, H, Sq, dv] or list(lse._shape) != [B, H, Sq]:
         raise RuntimeError("SDPA backward: out / lse do not belong to these inputs")
-    dq = TensorImpl([B, H, Sq, dk], "float32", "cuda")
-    dkk = TensorImpl([B, Hkv, Sk, dk], "float32", "cuda")
-    dvv = TensorImpl([B, Hkv, Sk, dv], "float32", "cuda")
+    if grad_dtype not in ("float32", "float16") or (grad_dtype == "float16" and window is None):
+        raise RuntimeError("SDPA backward: grad_dtype must be 'float32', or with a window 'float16'")
+    dq = TensorImpl([B, H, Sq, dk], grad_dtype, "cuda")
+    dkk = TensorImpl([B, Hkv, Sk, dk], grad_dtype, "cuda")
+    dvv = TensorImpl([B, Hkv, Sk, dv], grad_dtype, "cuda")
     lens, flags = None, _lib.TX_SDPA_OUT_F16 if out.dtype == "float16" else 0
+    if grad_dtype == "float16":
+        flags |= _lib.TX_BWD_GRADS_F16
     if kv_lens is not None:
         lens = _host_lens(kv_lens, B, "SDPA backward")
         flags |= _lib.TX_SDPA_KV_LENS_HOST
@@ -344,9 +353,28 @@ def scaled_dot_product_attention_backward(query, key, value, out, lse, grad, cau
         dq=dq.data_ptr, dk=dkk.data_ptr, dv=dvv.data_ptr, batch=B, q_heads=H, kv_heads=Hkv, seq_q=Sq, seq_k=Sk,
         d=dk, causal=int(bool(causal)), flags=flags, stream=None)
     lib = _lib.load()
-    _lib.check(lib.tx_sdpa_backward(ctypes.byref(desc)))
+    if window is None:
+        _lib.check(lib.tx_sdpa_backward(ctypes.byref(desc)))
+    else:
+        _lib.check(lib.tx_sdpa_window_backward(ctypes.byref(desc), ctypes.byref(window)))
     _lib.check(lib.tx_sdpa_finish(None))
     return dq, dkk, dvv
+
+
+def window_desc(window, sinks=0, align="start") -> "_lib.WindowDesc":
+    if align not in ("start", "end"):
+        raise RuntimeError("SDPA window: align must be 'start' or 'end'")
+    if int(window) < 1 or int(sinks) < 0:
+        raise RuntimeError("SDPA window: the window must hold a key at least, sinks must not be negative")
+    return _lib.WindowDesc(window=int(window), sinks=int(sinks), align_end=int(align == "end"))
+
+
+def scaled_dot_product_attention_window(query, key, value, window, sinks=0, align="start", kv_lens=None, flags=0,
+                                        out_dtype="float32", want_lse=False, sync=True):
+    """No reference counterpart: causal attention in which a row sees the last ``window`` keys up to its own position and the
+    first ``sinks`` ones.  Row i stands at position i, or with ``align="end"`` at len - Sq + i."""
+    return _forward(query, key, value, None, causal=True, kv_lens=kv_lens, flags=flags, out_dtype=out_dtype, want_lse=want_lse,
+                    sync=sync, window=window_desc(window, sinks, align), who="SDPA window")
 
 
 def scaled_dot_product_attention(query, key, value, mask=None) -> TensorImpl:

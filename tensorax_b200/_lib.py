@@ -22,6 +22,7 @@ TX_SDPA_OUT_F16 = 4
 TX_SDPA_F32_VIA_F16 = 8
 TX_SDPA_KV_LENS_HOST = 16
 TX_MHA_F16_ATTENTION = 32
+TX_BWD_GRADS_F16 = 64
 TX_KV_E4M3 = 0
 TX_KV_INT8 = 1
 TX_ERR_UNSUPPORTED = 5
@@ -42,6 +43,7 @@ EXPORTED_SYMBOLS = (
     "tx_sdpa_mma_profile_sections_cuda", "tx_sdpa_optimized_flash_profile_sections_cuda",
     "tx_selftest_wait_timeout", "tx_sdpa_forward_host_copies_only", "tx_sdpa_set_group_l2_bytes",
     "tx_mha_forward_f32",
+    "tx_sdpa_window_forward", "tx_sdpa_window_backward",
     "tx_kv_cache_write", "tx_kv_cache_read", "tx_kv_cache_attention",
 )
 
@@ -79,6 +81,11 @@ class MhaDesc(ctypes.Structure):
         ("batch", c_int64), ("seq_q", c_int64), ("seq_k", c_int64), ("embed", c_int64), ("heads", c_int64),
         ("causal", c_int32), ("flags", c_int32), ("stream", c_void_p),
     ]
+
+
+class WindowDesc(ctypes.Structure):
+    """Mirror of ``tx_window_desc``."""
+    _fields_ = [("window", c_int64), ("sinks", c_int64), ("align_end", c_int32), ("reserved", c_int32)]
 
 
 class KvCache(ctypes.Structure):
@@ -175,6 +182,8 @@ def load():
     lib.tx_sdpa_finish.argtypes = [c_void_p]
     lib.tx_sdpa_fp16_static_scratch.argtypes = [c_void_p] * 4 + [c_int64] * 6 + [c_int32, c_void_p, c_void_p]
     lib.tx_mha_forward_f32.argtypes = [ctypes.POINTER(MhaDesc)]
+    lib.tx_sdpa_window_forward.argtypes = [ctypes.POINTER(SdpaDesc), ctypes.POINTER(WindowDesc)]
+    lib.tx_sdpa_window_backward.argtypes = [ctypes.POINTER(SdpaBwdDesc), ctypes.POINTER(WindowDesc)]
     lib.tx_kv_cache_write.argtypes = [ctypes.POINTER(KvWriteDesc)]
     lib.tx_kv_cache_read.argtypes = [ctypes.POINTER(KvReadDesc)]
     lib.tx_kv_cache_attention.argtypes = [ctypes.POINTER(KvAttentionDesc)]

@@ -3,7 +3,7 @@
 // A row is one token of one K/V head: D codes of one byte that share a scale, kept in fp32.
 //   e4m3   scale = 2^e with the smallest e for which max|x| <= 448 * 2^e: dividing by it is exact, so a code is x rounded
 //          once, to four significant bits
-//   int8   scale = max|x| / 127, code = x / scale rounded to the nearest integer (IEEE division, ties to even)
+//   int8   scale = max|x| * (1/127) in fp32, code = x / scale rounded to the nearest integer (IEEE division, ties to even)
 // The scale is 2^-126 at least, so that it and its reciprocal are normal numbers.  A row with an infinity or a NaN in it
 // gets the scale NaN and zero codes: it reads back as NaN and makes NaN of the attention rows that see it, of no others.
 // 32-bit scales cost 4 bytes a row beside 64 to 256 of codes; powers of two would fit a byte, the int8 scales would not.
@@ -94,7 +94,7 @@ __device__ __forceinline__ float kv_scale(uint32_t top)
         const int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
         return __int_as_float(max(e, 1) << 23);
     } else {
-        return fmaxf(__fdiv_rn(__uint_as_float(top), 127.f), 1.17549435e-38f);
+        return fmaxf(__uint_as_float(top) * (1.f / 127.f), 1.17549435e-38f);
     }
 }
 

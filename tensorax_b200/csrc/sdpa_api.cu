@@ -364,7 +364,7 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem
     return TX_OK;
 }
 
-template <typename T, int DVC, bool PROF>
+template <typename T, int DVC, bool PROF, bool WINDOW>
 int launch_simt_t(const txb::SimtParams &p, cudaStream_t st)
 {
     dim3 grid((unsigned)((p.dv + 32 * DVC - 1) / (32 * DVC)),
@@ -376,28 +376,28 @@ int launch_simt_t(const txb::SimtParams &p, cudaStream_t st)
         int sms = 0, per_sm = fit.load(std::memory_order_relaxed);
         if (int rc = sm_count(&sms)) return rc;
         if (per_sm == 0) {
-            TX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, txb::sdpa_simt_kernel<T, DVC, PROF>, txb::SIMT_THREADS, 0));
+            TX_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, txb::sdpa_simt_kernel<T, DVC, PROF, WINDOW>, txb::SIMT_THREADS, 0));
             fit.store(per_sm = std::max(per_sm, 1), std::memory_order_relaxed);
         }
         const int64_t items = (int64_t)grid.x * grid.y * grid.z;
         grid = dim3((unsigned)std::min<int64_t>(items, (int64_t)sms * per_sm));
-        return launch_behind(txb::sdpa_simt_kernel<T, DVC, PROF>, grid, txb::SIMT_THREADS, 0, st, 1, p);
+        return launch_behind(txb::sdpa_simt_kernel<T, DVC, PROF, WINDOW>, grid, txb::SIMT_THREADS, 0, st, 1, p);
     }
-    txb::sdpa_simt_kernel<T, DVC, PROF><<<grid, txb::SIMT_THREADS, 0, st>>>(p);
+    txb::sdpa_simt_kernel<T, DVC, PROF, WINDOW><<<grid, txb::SIMT_THREADS, 0, st>>>(p);
     g_launches++;
     TX_CUDA(cudaGetLastError());
     return TX_OK;
 }
 
-template <typename T, bool PROF = false>
+template <typename T, bool PROF = false, bool WINDOW = false>
 int launch_simt(const txb::SimtParams &p, cudaStream_t st)
 {
     if (p.B * p.Hq > 65535) return fail(TX_ERR_UNSUPPORTED, "SDPA: batch*heads > 65535");
     if ((p.Sq + txb::SIMT_BR - 1) / txb::SIMT_BR > 65535) return fail(TX_ERR_UNSUPPORTED, "SDPA: seq_len_q too large");
-    if (p.dv <= 32) return launch_simt_t<T, 1, PROF>(p, st);
-    if (p.dv <= 64) return launch_simt_t<T, 2, PROF>(p, st);
-    if (p.dv <= 128) return launch_simt_t<T, 4, PROF>(p, st);
-    return launch_simt_t<T, 8, PROF>(p, st);   // wider heads: one CTA column per 256 value columns
+    if (p.dv <= 32) return launch_simt_t<T, 1, PROF, WINDOW>(p, st);
+    if (p.dv <= 64) return launch_simt_t<T, 2, PROF, WINDOW>(p, st);
+    if (p.dv <= 128) return launch_simt_t<T, 4, PROF, WINDOW>(p, st);
+    return launch_simt_t<T, 8, PROF, WINDOW>(p, st);   // wider heads: one CTA column per 256 value columns
 }
 
 // Elements (bit e = element e of each group of 16) whose exponential is evaluated by the FMA-pipe
@@ -408,10 +408,10 @@ constexpr int kPolyPairsD64 = 0x0303;
 // back-to-back runs move by 4-5 %: fewer special-function instructions also means a cooler part)
 constexpr int kPolyPairsD128 = 0x0003;
 
-int causal_group(const tx_sdpa_desc *d, int64_t items_per_slab, int64_t *group);
+int causal_group(const tx_sdpa_desc *d, int64_t items_per_slab, int64_t *group, const txb::WindowRule *win = nullptr);
 
 template <class Cfg>
-int launch_tc_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *prof = nullptr)
+int launch_tc_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *prof = nullptr, const txb::WindowRule *win = nullptr)
 {
     CUtensorMap tq, tk, tv, to;
     const bool out_f16 = (d->flags & TX_SDPA_OUT_F16) != 0;
@@ -435,9 +435,10 @@ int launch_tc_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *
     p.scale_log2 = (1.0f / std::sqrt((float)d->d_k)) * 1.4426950408889634f;
     p.prof = prof;
     p.skip_k_tile = -1;
+    if (win) p.win = *win;
     const int64_t n_tiles = (d->seq_q + Cfg::BM - 1) / Cfg::BM, slabs = d->batch * d->q_heads, zparts = d->d_v / Cfg::DV;
     int64_t group = 1;
-    if (int rc = causal_group(d, n_tiles * zparts, &group)) return rc;
+    if (int rc = causal_group(d, n_tiles * zparts, &group, win)) return rc;
     p.group = (int)group; p.n_pairs = (int)n_tiles; p.BH = (int)slabs;
     if (n_tiles * slabs * zparts > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA: more than 2^31 work items");
     if (int rc = allow_smem<txb::sdpa_tc_kernel<Cfg>>((int)Cfg::SMEM_BYTES)) return rc;
@@ -469,15 +470,17 @@ int launch_group(bool causal, int64_t slabs, int64_t items_per_slab, double byte
     return TX_OK;
 }
 
-int causal_group(const tx_sdpa_desc *d, int64_t items_per_slab, int64_t *group)
+// With a window all items but a slab's first few are equally long and neighbours share their keys: slab-major.
+int causal_group(const tx_sdpa_desc *d, int64_t items_per_slab, int64_t *group, const txb::WindowRule *win)
 {
     const int64_t ratio = d->q_heads / d->kv_heads;
-    return launch_group(d->causal != 0, d->batch * d->q_heads, items_per_slab,
+    return launch_group(d->causal != 0 && !win, d->batch * d->q_heads, items_per_slab,
                         2.0 * (double)d->seq_k * (double)(d->d_k + d->d_v) / (double)ratio, ratio, group);
 }
 
 template <class Cfg>
-int launch_pair_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *prof = nullptr, int skip_k_tile = -1)
+int launch_pair_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *prof = nullptr, int skip_k_tile = -1,
+                  const txb::WindowRule *win = nullptr)
 {
     CUtensorMap tq, tk, tv, to;
     const bool out_f16 = (d->flags & TX_SDPA_OUT_F16) != 0;
@@ -501,6 +504,7 @@ int launch_pair_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long
     p.scale_log2 = (1.0f / std::sqrt((float)d->d_k)) * 1.4426950408889634f;
     p.prof = prof;
     p.skip_k_tile = skip_k_tile;
+    if (win) p.win = *win;
     // Work items in launch order.  Slab-major (group = 1: a slab's CTAs, which share its K/V, start side by side)
     // unless the mask is causal: then the slabs are taken in groups, and inside a group every slab's longest items
     // come before any shorter one, so that the SMs do not end on a late slab's long items.  A group is as large as
@@ -513,7 +517,7 @@ int launch_pair_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long
     const int64_t n_pairs = (d->seq_q + 2 * Cfg::BM - 1) / (2 * Cfg::BM);
     const int64_t slabs = d->batch * d->q_heads;
     int64_t group = 1;
-    if (int rc = causal_group(d, n_pairs, &group)) return rc;
+    if (int rc = causal_group(d, n_pairs, &group, win)) return rc;
     p.group = (int)group;
     p.n_pairs = (int)n_pairs;
     p.BH = (int)slabs;
@@ -564,6 +568,18 @@ int launch_tc(const tx_sdpa_desc *d, cudaStream_t st, int *status, long long *pr
     return fail(TX_ERR_UNSUPPORTED, "SDPA: no tensor-core tile shape for d = %lld", (long long)d->d_k);
 }
 
+// The same shapes with a sliding window
+int launch_tc_window(const tx_sdpa_desc *d, cudaStream_t st, int *status, const txb::WindowRule *win)
+{
+    switch (d->d_k) {
+    case 64: return launch_pair_t<txb::PairCfg<64, 128, 4, kPolyPairsD64, false, false, false, true>>(d, st, status, nullptr, -1, win);
+    case 128: return launch_pair_t<txb::PairCfg<128, 128, 2, kPolyPairsD128, true, false, false, true>>(d, st, status, nullptr, -1, win);
+    case 256: return launch_tc_t<txb::TcCfg<256, 256, 64, 2, true, false, 0, 2, true, 128, false, true>>(d, st, status, nullptr, win);
+    case 512: return launch_tc_t<txb::TcCfg<512, 256, 64, 2, true, false, 0, 1, true, 160, true, true>>(d, st, status, nullptr, win);
+    }
+    return fail(TX_ERR_UNSUPPORTED, "SDPA: no tensor-core tile shape for d = %lld", (long long)d->d_k);
+}
+
 // Few query rows per K/V head (a decoding step): the kernel that reads the cache once and cuts the keys over a cluster.
 // fp16 up to 16 rows a head (CTAs of four rows each, side by side, read the same keys through L2; beyond that the
 // tensor-core kernel's 128-row tile is the better use of a CTA) and from one whole tile of keys on; fp32 up to 32 rows,
@@ -587,7 +603,7 @@ bool decode_eligible(const tx_sdpa_desc *d)
 }
 
 template <class Cfg>
-int launch_decode_t(const tx_sdpa_desc *d, cudaStream_t st, int *status)
+int launch_decode_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, const txb::WindowRule *win)
 {
     txb::DecodeParams p;
     p.q = d->q; p.k = d->k; p.v = d->v; p.mask = d->mask;
@@ -605,9 +621,14 @@ int launch_decode_t(const tx_sdpa_desc *d, cudaStream_t st, int *status)
     // costs 1.4 us more to start and merge) only where each then has four stages
     const int64_t items = d->batch * d->kv_heads * p.row_parts;
     if (items * Cfg::MAX_SPLITS > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA: more than 2^31 work items");
+    int64_t keys = d->seq_k;                                             // that a row can see
+    if (win) {
+        p.win = *win;
+        keys = std::min<int64_t>(keys, (int64_t)win->window + win->sinks + d->seq_q);
+    }
     int splits = 1;
-    const int most = d->seq_k >= 4 * Cfg::MAX_SPLITS * Cfg::KEYS ? Cfg::MAX_SPLITS : 8;
-    while (splits < most && items * splits * 2 <= Cfg::CTAS_PER_SM * sms && splits * Cfg::KEYS < d->seq_k) splits *= 2;
+    const int most = keys >= 4 * Cfg::MAX_SPLITS * Cfg::KEYS ? Cfg::MAX_SPLITS : 8;
+    while (splits < most && items * splits * 2 <= Cfg::CTAS_PER_SM * sms && splits * Cfg::KEYS < keys) splits *= 2;
     if (int rc = allow_smem<txb::sdpa_decode_kernel<Cfg>, true>((int)Cfg::SMEM)) return rc;
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
@@ -624,21 +645,21 @@ int launch_decode_t(const tx_sdpa_desc *d, cudaStream_t st, int *status)
     return TX_OK;
 }
 
-template <typename T, int D>
-int launch_decode_d(const tx_sdpa_desc *d, cudaStream_t st, int *status)
+template <typename T, int D, bool WINDOW>
+int launch_decode_d(const tx_sdpa_desc *d, cudaStream_t st, int *status, const txb::WindowRule *win)
 {
     const int64_t rows = d->q_heads / d->kv_heads * d->seq_q;
-    if (rows == 1) return launch_decode_t<txb::DecodeCfg<T, D, 1>>(d, st, status);
-    if (rows == 2) return launch_decode_t<txb::DecodeCfg<T, D, 2>>(d, st, status);
-    return launch_decode_t<txb::DecodeCfg<T, D, 4>>(d, st, status);
+    if (rows == 1) return launch_decode_t<txb::DecodeCfg<T, D, 1, WINDOW>>(d, st, status, win);
+    if (rows == 2) return launch_decode_t<txb::DecodeCfg<T, D, 2, WINDOW>>(d, st, status, win);
+    return launch_decode_t<txb::DecodeCfg<T, D, 4, WINDOW>>(d, st, status, win);
 }
 
-template <typename T>
-int launch_decode(const tx_sdpa_desc *d, cudaStream_t st, int *status)
+template <typename T, bool WINDOW = false>
+int launch_decode(const tx_sdpa_desc *d, cudaStream_t st, int *status, const txb::WindowRule *win = nullptr)
 {
-    if (d->d_k == 64) return launch_decode_d<T, 64>(d, st, status);
-    if (d->d_k == 128) return launch_decode_d<T, 128>(d, st, status);
-    return launch_decode_d<T, 256>(d, st, status);
+    if (d->d_k == 64) return launch_decode_d<T, 64, WINDOW>(d, st, status, win);
+    if (d->d_k == 128) return launch_decode_d<T, 128, WINDOW>(d, st, status, win);
+    return launch_decode_d<T, 256, WINDOW>(d, st, status, win);
 }
 
 // fp16 without a dense mask, at the shapes tc_eligible names
@@ -682,7 +703,8 @@ double bwd_together(const BwdWork &q, int zq, const BwdWork &k, int zk, int sms)
 }
 
 template <int D, class DqCfg, class DkvCfg>
-int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __half *dout_h, const float *delta, int *prepared)
+int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __half *dout_h, const float *delta, int *prepared,
+               const txb::WindowRule *win = nullptr)
 {
     txb::BwdParams p;
     p.lse = d->lse; p.delta = delta; p.kv_lens = lens_of(d->kv_lens, d->flags, d->batch);
@@ -697,12 +719,28 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
     p.split_q = p.split_k = 1;
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
+    if (win) { p.win = *win; p.grads_f16 = (d->flags & TX_BWD_GRADS_F16) ? 1 : 0; }
+    // With a window a key tile is seen by the rows of its window, the tiles of the sinks by all rows.  Where that makes them
+    // much longer than the others they get a launch of their own, cut over clusters, in front of the others.
+    int64_t sink_tiles = 0;
+    int split_sinks = 1;
     {
         auto up = [](int64_t n, int64_t by) { return (double)((n + by - 1) / by); };
-        const double ratio = (double)(d->q_heads / d->kv_heads), tq = up(d->seq_k, DqCfg::BN), tk = up(d->seq_q, DkvCfg::BQ) * ratio;
+        const double ratio = (double)(d->q_heads / d->kv_heads);
+        double tq = up(d->seq_k, DqCfg::BN), tk = up(d->seq_q, DkvCfg::BQ) * ratio;
+        if (win) {
+            const double all = tk;
+            tq = std::min(tq, up((int64_t)win->window + DqCfg::BM, DqCfg::BN) + up(std::min<int64_t>(win->sinks, d->seq_k), DqCfg::BN));
+            tk = std::min(tk, up((int64_t)win->window + DkvCfg::BMK, DkvCfg::BQ) * ratio);
+            if (win->sinks > 0 && all > 2.0 * tk) {
+                sink_tiles = std::min<int64_t>((win->sinks + DkvCfg::BMK - 1) / DkvCfg::BMK, (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK);
+                while (split_sinks < 8 && all / split_sinks > tk) split_sinks *= 2;
+            }
+        }
+        const bool uneven = d->causal && !win;           // half of the tiles on average
         // a dK/dV tile against a dQ tile, one CTA per SM: 1.2 and 1.7 us at d = 128, 1.8 and 2.2 at d = 256
-        const BwdWork q = {up(d->seq_q, DqCfg::BM) * (double)(d->batch * d->q_heads), tq, d->causal ? 0.5 * (tq + 1) : tq, 1.0};
-        const BwdWork k = {up(d->seq_k, DkvCfg::BMK) * (double)(d->batch * d->kv_heads * DkvCfg::ZS), tk, d->causal ? 0.5 * (tk + ratio) : tk,
+        const BwdWork q = {up(d->seq_q, DqCfg::BM) * (double)(d->batch * d->q_heads), tq, uneven ? 0.5 * (tq + 1) : tq, 1.0};
+        const BwdWork k = {up(d->seq_k, DkvCfg::BMK) * (double)(d->batch * d->kv_heads * DkvCfg::ZS), tk, uneven ? 0.5 * (tk + ratio) : tk,
                            D == 128 ? 0.7 : 0.82};
         p.split_q = bwd_split(q, sms, DqCfg::CTAS_PER_SM);
         p.split_k = bwd_split(k, sms, DkvCfg::CTAS_PER_SM);
@@ -725,7 +763,7 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
         const int64_t ratio = d->q_heads / d->kv_heads;
         int64_t group = 1;
         // (beyond 32 waves the slab-major order was the better one here: B8 Hq32 Hkv8 S4096 d128 4.24 against 4.35 ms)
-        if (int rc = launch_group(d->causal != 0, slabs, items, 4.0 * (double)d->seq_k * (double)D / (double)ratio, ratio, &group, 32))
+        if (int rc = launch_group(d->causal != 0 && !win, slabs, items, 4.0 * (double)d->seq_k * (double)D / (double)ratio, ratio, &group, 32))
             return rc;
         p.group_q = (int)group; p.items_q = (int)items; p.slabs_q = (int)slabs;
         if (items * slabs * p.split_q > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA backward: more than 2^31 work items");
@@ -742,10 +780,22 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
         if (int rc = allow_smem<txb::sdpa_bwd_dkv_kernel<DkvCfg>>((int)DkvCfg::SMEM_BYTES)) return rc;
         // 1-D grid: (slab of (batch, K/V head)) x key tile x column part; a slab's CTAs stream the Q and dO of its
         // query heads
-        const int64_t items = (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK, slabs = d->batch * d->kv_heads;
+        const int64_t slabs = d->batch * d->kv_heads, items = (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK - sink_tiles;
         const int64_t ratio = d->q_heads / d->kv_heads;
+        if (sink_tiles > 0) {
+            txb::BwdParams ps = p;
+            ps.group_k = 1; ps.items_k = (int)sink_tiles; ps.slabs_k = (int)slabs; ps.split_k = split_sinks;
+            ps.early_k = items > 0;
+            const int64_t ctas = sink_tiles * slabs * DkvCfg::ZS * split_sinks;
+            if (ctas > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA backward: more than 2^31 work items");
+            if (int rc = launch_behind(txb::sdpa_bwd_dkv_kernel<DkvCfg>, dim3((unsigned)ctas), DkvCfg::THREADS, DkvCfg::SMEM_BYTES, st,
+                                       split_sinks, tq, tdo, tk, tv, ps))
+                return rc;
+            if (items == 0) return TX_OK;
+            p.first_k = (int)sink_tiles;
+        }
         int64_t group = 1;
-        if (int rc = launch_group(d->causal != 0, slabs, items * DkvCfg::ZS, 4.0 * (double)ratio * (double)d->seq_q * (double)D, 1, &group, 32))
+        if (int rc = launch_group(d->causal != 0 && !win, slabs, items * DkvCfg::ZS, 4.0 * (double)ratio * (double)d->seq_q * (double)D, 1, &group, 32))
             return rc;
         p.group_k = (int)group; p.items_k = (int)items; p.slabs_k = (int)slabs;
         const int64_t ctas = items * slabs * DkvCfg::ZS * p.split_k;
@@ -824,7 +874,7 @@ void fill_simt_params(txb::SimtParams *p, const tx_sdpa_desc *d)
 // `zeroed`: three words of device memory that are zero behind a launch of this library that lets its successor start under
 // its end (the layer); without them the call brings its own.
 template <class Cfg>
-int launch_x3_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed)
+int launch_x3_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed, const txb::WindowRule *win)
 {
     const int64_t rows_q = d->batch * d->q_heads * d->seq_q, rows_k = d->batch * d->kv_heads * d->seq_k;
     const int64_t dk8 = (d->d_k + 7) / 8 * 8, dv8 = (d->d_v + 7) / 8 * 8;       // row length of the fp16 copies
@@ -888,7 +938,8 @@ int launch_x3_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed
         p.scale_log2 = p.scale * 1.4426950408889634f;
         const int64_t n_tiles = (d->seq_q + Cfg::BM - 1) / Cfg::BM;
         int64_t group = 1;
-        if (int r = causal_group(d, n_tiles, &group)) return r;
+        if (int r = causal_group(d, n_tiles, &group, win)) return r;
+        if (win) p.win = *win;
         p.group = (int)group; p.n_tiles_q = (int)n_tiles; p.BH = (int)sq;
         if (n_tiles * sq > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA: more than 2^31 work items");
         if (int r = allow_smem<txb::sdpa_tc_x3_kernel<Cfg>>((int)Cfg::SMEM_BYTES)) return r;
@@ -899,6 +950,10 @@ int launch_x3_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed
         txb::SimtParams sp2;
         fill_simt_params(&sp2, d);
         sp2.only_if = range;
+        if constexpr (Cfg::WINDOW) {
+            sp2.win = *win;
+            return launch_simt<float, false, true>(sp2, st);
+        }
         return launch_simt<float>(sp2, st);
     };
     rc = body();
@@ -906,10 +961,11 @@ int launch_x3_t(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed
     return rc;
 }
 
-int launch_x3(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed = nullptr)
+int launch_x3(const tx_sdpa_desc *d, cudaStream_t st, int *status, int *zeroed = nullptr, const txb::WindowRule *win = nullptr)
 {
-    auto on = [&](auto cfg) { return launch_x3_t<decltype(cfg)>(d, st, status, zeroed); };
+    auto on = [&](auto cfg) { return launch_x3_t<decltype(cfg)>(d, st, status, zeroed, win); };
     const bool narrow = d->d_k <= 64 && d->d_v <= 64;
+    if (win) return narrow ? on(txb::X3Cfg<64, 4, false, true>{}) : on(txb::X3Cfg<128, 2, false, true>{});
     if (d->mask) return narrow ? on(txb::X3Cfg<64, 2, true>{}) : on(txb::X3Cfg<128, 2, true>{});
     return narrow ? on(txb::X3Cfg<64, 4>{}) : on(txb::X3Cfg<128, 2>{});
 }
@@ -954,6 +1010,43 @@ int forward(const tx_sdpa_desc *d)
     if (int rc = validate(d)) return rc;
     if (int rc = ensure_device()) return rc;
     return with_device_lens(d, forward_launch);
+}
+
+int window_rule(const tx_window_desc *w, txb::WindowRule *rule)
+{
+    if (!w) return fail(TX_ERR_INVALID, "SDPA window: null descriptor");
+    if (w->window < 1 || w->sinks < 0) return fail(TX_ERR_INVALID, "SDPA window: the window must hold a key at least, sinks must not be negative");
+    if (w->align_end != 0 && w->align_end != 1) return fail(TX_ERR_INVALID, "SDPA window: align_end must be 0 or 1");
+    // sequences have less than 2^30 positions: beyond that it is all the same
+    rule->window = (int)std::min<int64_t>(w->window, 0x3fffffffLL);
+    rule->sinks = (int)std::min<int64_t>(w->sinks, 0x3fffffffLL);
+    rule->align_end = w->align_end;
+    return TX_OK;
+}
+
+int window_forward(const tx_sdpa_desc *d, const tx_window_desc *w)
+{
+    if (int rc = validate(d)) return rc;
+    txb::WindowRule rule;
+    if (int rc = window_rule(w, &rule)) return rc;
+    if (!d->causal || d->mask) return fail(TX_ERR_INVALID, "SDPA window: a window is causal (desc.causal nonzero) and takes no dense mask");
+    if (d->flags & ~(TX_SDPA_FORCE_SIMT | TX_SDPA_OUT_F16 | TX_SDPA_KV_LENS_HOST)) return fail(TX_ERR_INVALID, "SDPA window: unknown flags");
+    if (int rc = ensure_device()) return rc;
+    return with_device_lens(d, [&](const tx_sdpa_desc *e) -> int {
+        cudaStream_t st = static_cast<cudaStream_t>(e->stream);
+        const Route route = route_of(e);
+        if (route == Route::CudaCores) {
+            txb::SimtParams p;
+            fill_simt_params(&p, e);
+            p.win = rule;
+            return e->dtype == TX_DTYPE_F16 ? launch_simt<__half, false, true>(p, st) : launch_simt<float, false, true>(p, st);
+        }
+        int *status = nullptr;
+        if (int rc = status_word(&status)) return rc;
+        if (route == Route::Decode)
+            return e->dtype == TX_DTYPE_F16 ? launch_decode<__half, true>(e, st, status, &rule) : launch_decode<float, true>(e, st, status, &rule);
+        return route == Route::TensorCores ? launch_tc_window(e, st, status, &rule) : launch_x3(e, st, status, nullptr, &rule);
+    });
 }
 
 int finish(cudaStream_t st)
@@ -1735,9 +1828,24 @@ int tx_selftest_wait_timeout(const tx_sdpa_desc *d, int32_t skip_k_tile)
     return finish(st);
 }
 
-static int backward_launch(const tx_sdpa_bwd_desc *d);
+static int backward_launch(const tx_sdpa_bwd_desc *d, const txb::WindowRule *win);
+static int backward(const tx_sdpa_bwd_desc *d, const tx_window_desc *w);
 
-int tx_sdpa_backward(const tx_sdpa_bwd_desc *d)
+int tx_sdpa_backward(const tx_sdpa_bwd_desc *d) { return backward(d, nullptr); }
+
+int tx_sdpa_window_forward(const tx_sdpa_desc *d, const tx_window_desc *w)
+{
+    TX_NVTX_RANGE("sdpa.window.forward");
+    return window_forward(d, w);
+}
+
+int tx_sdpa_window_backward(const tx_sdpa_bwd_desc *d, const tx_window_desc *w)
+{
+    if (!w) return fail(TX_ERR_INVALID, "SDPA window: null descriptor");
+    return backward(d, w);
+}
+
+static int backward(const tx_sdpa_bwd_desc *d, const tx_window_desc *w)
 {
     if (!d) return fail(TX_ERR_INVALID, "SDPA backward: null descriptor");
     if (!d->q || !d->k || !d->v || !d->out || !d->dout || !d->lse || !d->dq || !d->dk || !d->dv)
@@ -1754,11 +1862,17 @@ int tx_sdpa_backward(const tx_sdpa_bwd_desc *d)
     auto al = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; };
     if (!al(d->q) || !al(d->k) || !al(d->v) || !al(d->out) || !al(d->dout) || !al(d->dq) || !al(d->dk) || !al(d->dv))
         return fail(TX_ERR_INVALID, "SDPA backward: pointers must be 16-byte aligned");
+    txb::WindowRule rule;
+    if (w) {
+        if (int rc = window_rule(w, &rule)) return rc;
+        if (!d->causal) return fail(TX_ERR_INVALID, "SDPA window: a window is causal (desc.causal nonzero)");
+        if (d->flags & ~(TX_SDPA_OUT_F16 | TX_SDPA_KV_LENS_HOST | TX_BWD_GRADS_F16)) return fail(TX_ERR_INVALID, "SDPA window: unknown flags");
+    }
     if (int rc = ensure_device()) return rc;
-    return with_device_lens(d, backward_launch);
+    return with_device_lens(d, [&](const tx_sdpa_bwd_desc *e) { return backward_launch(e, w ? &rule : nullptr); });
 }
 
-static int backward_launch(const tx_sdpa_bwd_desc *d)
+static int backward_launch(const tx_sdpa_bwd_desc *d, const txb::WindowRule *win)
 {
     int *status = nullptr;
     if (int rc = status_word(&status)) return rc;
@@ -1790,15 +1904,18 @@ static int backward_launch(const tx_sdpa_bwd_desc *d)
         // per SM and two row warpgroups, config-2 size).
         // d = 128: one CTA per SM for both, two row warpgroups, 128-key / 64-query tiles (all of tensor memory).
         if (d->d == 64)
-            rc = launch_bwd<64, txb::BwdDqCfg<64, 64, 3, 1, 2>, txb::BwdDkvCfg<64, 64, 3, 1, true, 2>>(d, st, status, dout_h, delta, prepared);
+            rc = win ? launch_bwd<64, txb::BwdDqCfg<64, 64, 3, 1, 2, true>, txb::BwdDkvCfg<64, 64, 3, 1, true, 2, 1, true>>(d, st, status, dout_h, delta, prepared, win)
+                     : launch_bwd<64, txb::BwdDqCfg<64, 64, 3, 1, 2>, txb::BwdDkvCfg<64, 64, 3, 1, true, 2>>(d, st, status, dout_h, delta, prepared);
         else if (d->d == 128)
-            rc = launch_bwd<128, txb::BwdDqCfg<128, 128, 3, 2, 2>, txb::BwdDkvCfg<128, 64, 3, 2, false, 3>>(d, st, status, dout_h, delta, prepared);
+            rc = win ? launch_bwd<128, txb::BwdDqCfg<128, 128, 3, 2, 2, true>, txb::BwdDkvCfg<128, 64, 3, 2, false, 3, 1, true>>(d, st, status, dout_h, delta, prepared, win)
+                     : launch_bwd<128, txb::BwdDqCfg<128, 128, 3, 2, 2>, txb::BwdDkvCfg<128, 64, 3, 2, false, 3>>(d, st, status, dout_h, delta, prepared);
         else
             // d = 256: dQ alone takes 256 tensor-memory columns (64-key tiles, single V stage: 224 KB of shared
             // memory); two CTAs per key tile each own 128 columns of dK and dV, with 32-query tiles so that two
             // stages each of Q and dO fit beside the resident K and V (a stage stays occupied from its first
             // read to its second, so one stage per ring would deadlock the MMA warp).
-            rc = launch_bwd<256, txb::BwdDqCfg<256, 64, 2, 1, 1>, txb::BwdDkvCfg<256, 32, 2, 1, false, 2, 2>>(d, st, status, dout_h, delta, prepared);
+            rc = win ? launch_bwd<256, txb::BwdDqCfg<256, 64, 2, 1, 1, true>, txb::BwdDkvCfg<256, 32, 2, 1, false, 2, 2, true>>(d, st, status, dout_h, delta, prepared, win)
+                     : launch_bwd<256, txb::BwdDqCfg<256, 64, 2, 1, 1>, txb::BwdDkvCfg<256, 32, 2, 1, false, 2, 2>>(d, st, status, dout_h, delta, prepared);
     }
     pool_free(ws, st);        // ordered after the kernels on `st`
     return rc;

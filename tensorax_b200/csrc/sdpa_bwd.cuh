@@ -56,6 +56,11 @@ struct BwdParams {
     // CTAs (a thread-block cluster, neighbours in the 1-D grid) that share one work item: CTA z of `split_*` takes the
     // item's tiles z, z + split, z + 2 split ... and the cluster adds the partial gradients in rank order.
     int split_q, split_k;
+    // WINDOW instantiations (window.cuh).  first_k: key tile of the dK/dV launch's item 0 (its slabs have items_k tiles from
+    // there on); early_k: the launch behind this one reads nothing of it and may start beside it.
+    WindowRule win;
+    int grads_f16 = 0;        // dq, dk, dv are fp16
+    int first_k = 0, early_k = 0;
 };
 
 // ------------------------------------------------------------------ result
@@ -125,6 +130,40 @@ __device__ __forceinline__ void store_grad(const uint8_t *tile, float *dst, int6
     }
 }
 
+// store_grad into fp16 (saturating at nothing: a gradient beyond fp16's range becomes infinite, as a cast would make it)
+template <int W, int THREADS>
+__device__ __forceinline__ void store_grad_half(const uint8_t *tile, __half *dst, int64_t ld, int rows_ok, int rank, int split,
+                                                bool filled, int tid)
+{
+    namespace cg = cooperative_groups;
+    constexpr int C = W / 8;
+    const int rows = 128 / split, r0 = rank * rows;
+#pragma unroll 4
+    for (int i = tid; i < rows * C; i += THREADS) {
+        const int r = r0 + i / C, c = i % C;
+        if (r >= rows_ok) break;
+        float4 v[2] = {};
+        if (!filled) {
+            cg::cluster_group cluster = cg::this_cluster();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint8_t *at = tile + grad_chunk<W>(r, 2 * c + e);
+                if (split == 1) { v[e] = *reinterpret_cast<const float4 *>(at); continue; }
+                float4 part[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z)
+                    if (z < split) part[z] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(at, z));
+                v[e] = part[0];
+#pragma unroll
+                for (int z = 1; z < 8; ++z)
+                    if (z < split) { v[e].x += part[z].x; v[e].y += part[z].y; v[e].z += part[z].z; v[e].w += part[z].w; }
+            }
+        }
+        *reinterpret_cast<uint4 *>(dst + (int64_t)r * ld + c * 8) =
+            make_uint4(ptx::pack_half2(v[0].x, v[0].y), ptx::pack_half2(v[0].z, v[0].w), ptx::pack_half2(v[1].x, v[1].y), ptx::pack_half2(v[1].z, v[1].w));
+    }
+}
+
 // ------------------------------------------------------------------ preprocess
 // dO fp32 -> fp16 (MMA operand) and delta = rowsum(dO o O).  Bound: HBM (10 d + 4 or 8 d + 4 bytes a row).  Sixteen lanes a row
 // at d = 64, 32 otherwise, four values a lane and step; a warp requests two steps of rows at a time.  One row a warp and
@@ -178,8 +217,9 @@ __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restr
 // WGS: row warpgroups (4 warps, one thread per TMEM lane each); with 2, each takes half of a tile's columns.
 // NS / NSV: depth of the K / V ring.  A K stage is read twice (S = Q K^T, later dQ += dS K) and only
 // then freed, so its ring is one deeper than V's, whose stage goes back right after dP = dO V^T.
-template <int D_, int BN_, int NS_, int WGS_ = 1, int NSV_ = 2>
+template <int D_, int BN_, int NS_, int WGS_ = 1, int NSV_ = 2, bool WINDOW_ = false>
 struct BwdDqCfg {
+    static constexpr bool WINDOW = WINDOW_;
     static constexpr int D = D_, BN = BN_, NS = NS_, NSV = NSV_, BM = 128, WGS = WGS_;
     static constexpr int CW = BN / WGS;                      // tile columns per warpgroup
     static constexpr int THREADS = 64 + 128 * WGS;
@@ -239,7 +279,10 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     kv_limit = p.kv_lens.limit(b, kv_limit);
     int kv_end = kv_limit;
     if (p.causal) kv_end = min(kv_end, q0 + BM);
-    const int n_all = (kv_end + BN - 1) / BN;
+    const int pos0 = Cfg::WINDOW ? q0 + p.win.offset(kv_limit, p.Sq) : q0;
+    const WindowWalk<BN> walk(p.win, kv_limit, pos0, BM);
+    const int n_all = Cfg::WINDOW ? walk.count() : (kv_end + BN - 1) / BN;
+    auto first_key = [&](int j) { return (Cfg::WINDOW ? walk.tile(rank + j * split) : rank + j * split) * BN; };
     const int n_tiles = n_all > rank ? (n_all - rank + split - 1) / split : 0;      // tiles rank, rank + split, ...
 
     auto load_k = [&](int j) {
@@ -248,7 +291,7 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
         for (int pn = 0; pn < Cfg::KP; ++pn)
             ptx::tma_load_3d(k_s + s * Cfg::KV_BYTES + pn * Cfg::KV_PANEL, &tm_k, k_full + 8 * s, pn * 64,
-                             (rank + j * split) * BN, kvh);
+                             first_key(j), kvh);
     };
     auto load_v = [&](int j) {
         const int s = j % NSV;
@@ -256,7 +299,7 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
         for (int pn = 0; pn < Cfg::KP; ++pn)
             ptx::tma_load_3d(v_s + s * Cfg::KV_BYTES + pn * Cfg::KV_PANEL, &tm_v, v_full + 8 * s, pn * 64,
-                             (rank + j * split) * BN, kvh);
+                             first_key(j), kvh);
     };
     if (tid == 0) {
         *abort_flag = 0;
@@ -424,7 +467,7 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (lane == 0) ptx::mbar_arrive(bar);
         };
         for (int j = 0; j < n_tiles && ok; ++j) {
-            const int kv0 = (rank + j * split) * BN + c0;
+            const int kv0 = first_key(j) + c0;
             ok = ptx::mbar_wait(s_full, (uint32_t)j & 1u, abort_flag);
             if (!ok) break;
             ptx::tc_fence_after_sync();
@@ -438,8 +481,10 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             ptx::reg_fence_cols<CW>(sv);
             ptx::reg_fence_cols<CW>(dpv);
             arrive_warp(s_free);
-            const bool need_mask = (kv0 + CW > kv_limit) || (p.causal && (kv0 + CW - 1 > q0));
+            const bool need_mask = Cfg::WINDOW ? window_edge(p.win, kv_limit, pos0, BM, kv0, CW)
+                                               : (kv0 + CW > kv_limit) || (p.causal && (kv0 + CW - 1 > q0));
             const int lim = min(kv_limit - kv0, p.causal ? row - kv0 + 1 : CW);
+            const WindowColumns seen(p.win, kv_limit, pos0 + r, kv0);
             uint32_t pk[CW / 2];
             // packed fp32 pairs: x = s*c - lse, t = dP*scale - D*scale, dS = P*t
             const float2 c2 = make_float2(p.scale_log2, p.scale_log2), nl2 = make_float2(-lse, -lse);
@@ -448,18 +493,26 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             for (int i = 0; i < CW; i += 2) {
                 const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), c2, nl2);
                 float2 pr = make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
-                if (need_mask) {                 // visible keys of this row are a prefix of the tile: [0, lim)
+                if (!Cfg::WINDOW && need_mask) { // visible keys of this row are a prefix of the tile: [0, lim)
                     pr.x = ptx::zero_unless_lt(pr.x, i, lim);
                     pr.y = ptx::zero_unless_lt(pr.y, i + 1, lim);
                 }
                 const float2 tt = __ffma2_rn(make_float2(__uint_as_float(dpv[i]), __uint_as_float(dpv[i + 1])), s2, nd2);
-                const float2 ds = __fmul2_rn(pr, tt);
+                float2 ds = __fmul2_rn(pr, tt);
+                if (Cfg::WINDOW && need_mask) {  // the product: a row that sees nothing has no statistics either
+                    ds.x = zero_unless_seen(ds.x, i, seen);
+                    ds.y = zero_unless_seen(ds.y, i + 1, seen);
+                }
                 pk[i / 2] = ptx::pack_half2(ds.x, ds.y);
             }
             if (j > 0) {
                 ok = ptx::mbar_wait(dq_done, (uint32_t)(j - 1) & 1u, abort_flag);   // dS of tile j-1 consumed
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
+            }
+            if (Cfg::WINDOW && first_key(j) + BN > kv_limit) {      // what lies behind the sequence's last key, for dS K
+                zero_stage_rows<BN, 128 * Cfg::WGS>(smem + Cfg::OFF_K + (j % NS) * Cfg::KV_BYTES, Cfg::KP, kv_limit - first_key(j), tid - 64);
+                ptx::fence_proxy_async_smem();
             }
             ptx::tmem_st_cols<CW / 2>(t_ds, pk);
             ptx::tmem_wait_st();
@@ -484,9 +537,13 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     if (split > 1) cooperative_groups::this_cluster().sync();
     else __syncthreads();
     // a row without any visible key: the forward row is 0/0, and so is its gradient
-    if (*abort_flag == 0)
+    // (with a window, where that happens to padding beside rows that do: nothing)
+    if (Cfg::WINDOW && p.grads_f16 && *abort_flag == 0)
+        store_grad_half<D, Cfg::THREADS>(smem, reinterpret_cast<__half *>(p.dq) + ((size_t)bh * p.Sq + q0) * D, D, p.Sq - q0, rank, split,
+                                         n_all == 0, tid);
+    else if (*abort_flag == 0)
         store_grad<D, Cfg::THREADS>(smem, p.dq + ((size_t)bh * p.Sq + q0) * D, D, p.Sq - q0, rank, split, n_all == 0,
-                                    __int_as_float(0x7fc00000), tid);
+                                    Cfg::WINDOW ? 0.f : __int_as_float(0x7fc00000), tid);
     else
         for (int i = 0; i < 64; ++i) __nanosleep(2000);
     if (warp == 1) {
@@ -503,8 +560,10 @@ sdpa_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 // dK / dV) and stay occupied until the second read is done.
 // ZS: CTAs (side by side in the 1-D grid) that share one key tile, each accumulating D/ZS columns of dK and dV (both form the whole
 // S^T and dP^T): at d = 256 the two accumulators of one CTA would need all 512 tensor-memory columns.
-template <int D_, int BQ_, int NS_, int WGS_ = 1, bool PS_SMEM_ = false, int NSD_ = NS_, int ZS_ = 1>
+template <int D_, int BQ_, int NS_, int WGS_ = 1, bool PS_SMEM_ = false, int NSD_ = NS_, int ZS_ = 1,
+          bool WINDOW_ = false>
 struct BwdDkvCfg {
+    static constexpr bool WINDOW = WINDOW_;
     static constexpr int D = D_, BQ = BQ_, NS = NS_, NSD = NSD_, BMK = 128, WGS = WGS_, ZS = ZS_;
     static constexpr int DA = D / ZS;                        // gradient columns this CTA accumulates
     static constexpr bool PS_SMEM = PS_SMEM_;
@@ -564,7 +623,7 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const int span = p.group_k * p.items_k;
     const int grp = item / span, rem = item % span;
     const int in_grp = min(p.group_k, p.slabs_k - grp * p.group_k);
-    const int key0 = (rem / in_grp) * BMK;
+    const int key0 = (rem / in_grp + (Cfg::WINDOW ? p.first_k : 0)) * BMK;
     const int col0 = (part % Cfg::ZS) * DA;          // first dK / dV column of this CTA
     const int kvh = grp * p.group_k + rem % in_grp;             // b * Hkv + kv head
     const int b = kvh / p.Hkv;
@@ -574,8 +633,16 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     kv_limit = p.kv_lens.limit(b, kv_limit);
     const int nq = (p.Sq + BQ - 1) / BQ;
     // causal: query rows below the tile's first key see none of its keys
-    const int i_start = p.causal ? min(key0 / BQ, nq) : 0;
-    const int per_head = (key0 < kv_limit) ? nq - i_start : 0;  // a tile beyond the valid keys gets zero gradients
+    const int off = Cfg::WINDOW ? p.win.offset(kv_limit, p.Sq) : 0;
+    const int i_start = p.causal ? min(max(key0 - off, 0) / BQ, nq) : 0;
+    // window: no row behind the last key's window sees the tile, unless it holds a sink
+    int i_end = nq;
+    if (Cfg::WINDOW && key0 >= p.win.sinks) {
+        const int64_t rows_end = (int64_t)key0 + BMK - 1 + p.win.window - off;
+        i_end = rows_end <= 0 ? i_start : (int)max((int64_t)i_start, min((int64_t)nq, (rows_end + BQ - 1) / BQ));
+    }
+    const int per_head = (key0 < kv_limit) ? i_end - i_start : 0;  // a tile beyond the valid keys gets zero gradients
+    if (Cfg::WINDOW && p.early_k) ptx::grid_trigger();
     const int n_all = per_head * group;
     const int n_it = n_all > rank ? (n_all - rank + split - 1) / split : 0;         // tiles rank, rank + split, ...
     auto tile_of = [&](int t, int &head, int &row0) {           // query head and first query row of this CTA's tile t
@@ -823,7 +890,11 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             ptx::reg_fence_cols<CW>(dpv);
             arrive_warp(s_free);
             const int qc0 = qr0 + c0;               // first query of this warpgroup's columns
-            const bool need_mask = p.causal && (key0 + BMK - 1 > qc0);
+            // columns of the tile whose queries see this key: from its own position on, as far as its window goes
+            const int seen_lo = key - off - qc0, seen_hi = key < p.win.sinks ? CW : min(CW, seen_lo + p.win.window);
+            const bool need_mask = Cfg::WINDOW ? (key0 + BMK - 1 > off + qc0 || key0 + BMK > kv_limit ||
+                                                  (off + qc0 + CW - 1 >= key0 + p.win.window && key0 + BMK > p.win.sinks))
+                                               : p.causal && (key0 + BMK - 1 > qc0);
             const int key_lo = key - qc0 - 1;
             uint32_t pp[CW / 2], pd[CW / 2];
             const float2 c2 = make_float2(p.scale_log2, p.scale_log2), s2 = make_float2(p.scale, p.scale);
@@ -834,14 +905,21 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const float2 dl = *reinterpret_cast<const float2 *>(st_delta + c0 + i);
                 const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), c2, l2);
                 float2 pr = make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
-                if (!key_ok) pr = make_float2(0.f, 0.f);
-                if (need_mask) {                 // query qc0 + i sees this key when key <= qc0 + i
+                if (!Cfg::WINDOW && !key_ok) pr = make_float2(0.f, 0.f);
+                if (!Cfg::WINDOW && need_mask) { // query qc0 + i sees this key when key <= qc0 + i
                     pr.x = ptx::zero_unless_lt(pr.x, key_lo, i);
                     pr.y = ptx::zero_unless_lt(pr.y, key_lo, i + 1);
                 }
                 const float2 tt = __ffma2_rn(make_float2(__uint_as_float(dpv[i]), __uint_as_float(dpv[i + 1])), s2,
                                              dl);
-                const float2 ds = __fmul2_rn(pr, tt);
+                float2 ds = __fmul2_rn(pr, tt);
+                if (Cfg::WINDOW && need_mask) {  // both: a query that sees nothing has no statistics, a key behind the last no value
+                    const int hi = key_ok ? seen_hi : -1;
+                    pr.x = zero_unless_within(pr.x, i, seen_lo, hi);
+                    pr.y = zero_unless_within(pr.y, i + 1, seen_lo, hi);
+                    ds.x = zero_unless_within(ds.x, i, seen_lo, hi);
+                    ds.y = zero_unless_within(ds.y, i + 1, seen_lo, hi);
+                }
                 pp[i / 2] = ptx::pack_half2(pr.x, pr.y);
                 pd[i / 2] = ptx::pack_half2(ds.x, ds.y);
             }
@@ -889,10 +967,15 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     if (*abort_flag == 0) {
         // keys no query sees: zero gradients -- unless the batch element has no valid key at
         // all, where the forward rows are 0/0 and the reference's rule propagates NaN to every gradient
-        const float fill = kv_limit == 0 ? __int_as_float(0x7fc00000) : 0.f;
+        const float fill = kv_limit == 0 && !Cfg::WINDOW ? __int_as_float(0x7fc00000) : 0.f;
         const size_t gbase = ((size_t)kvh * p.Sk + key0) * D + col0;
+        if (Cfg::WINDOW && p.grads_f16) {
+            store_grad_half<DA, Cfg::THREADS>(smem, reinterpret_cast<__half *>(p.dk) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid);
+            store_grad_half<DA, Cfg::THREADS>(smem + BMK * DA * 4, reinterpret_cast<__half *>(p.dv) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid);
+        } else {
         store_grad<DA, Cfg::THREADS>(smem, p.dk + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid);
         store_grad<DA, Cfg::THREADS>(smem + BMK * DA * 4, p.dv + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid);
+        }
     } else {
         for (int i = 0; i < 64; ++i) __nanosleep(2000);
     }

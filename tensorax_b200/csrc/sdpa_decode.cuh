@@ -27,6 +27,7 @@
 #include <cooperative_groups.h>
 
 #include "ptx.cuh"
+#include "window.cuh"
 
 namespace txb {
 
@@ -44,10 +45,12 @@ struct DecodeParams {
     int row_parts;            // CTAs (per split) that share them, R rows each
     int causal, out_f16;
     float scale;              // 1/sqrt(d)
+    WindowRule win;           // WINDOW instantiations
 };
 
-template <typename T_, int D_, int R_>
+template <typename T_, int D_, int R_, bool WINDOW_ = false>
 struct DecodeCfg {
+    static constexpr bool WINDOW = WINDOW_;                              // sliding window with sinks (window.cuh)
     using T = T_;
     static constexpr int D = D_, R = R_, WARPS = 7;
     static constexpr int VEC = 16 / (int)sizeof(T);                      // elements of one 16-byte load
@@ -119,7 +122,17 @@ sdpa_decode_kernel(const DecodeParams p)
     const int kvh = item / p.row_parts, row0 = (item % p.row_parts) * R; // (batch, K/V head), first of this CTA's rows
     const int b = kvh / p.Hkv;
     int limit = p.kv_lens.limit(b, p.Sk);
-    if (p.causal) limit = min(limit, p.Sq);
+    // With a window the keys are numbered without those that no row sees: number c is key c, or c + skip behind the sinks
+    // in front of the first row's window.
+    const int last = limit, off = Cfg::WINDOW ? p.win.offset(limit, p.Sq) : 0;
+    int s_end = 0, skip = 0;
+    if constexpr (Cfg::WINDOW) {
+        limit = max(0, min(limit, off + p.Sq));
+        const int first = min(max(0, off - p.win.window + 1), limit);
+        s_end = min(p.win.sinks, first);
+        skip = first - s_end;
+        limit -= skip;
+    } else if (p.causal) limit = min(limit, p.Sq);
     // equal shares of the visible keys, whole warp rounds each
     const int share = ((limit + splits - 1) / splits + Cfg::KEYS - 1) / Cfg::KEYS * Cfg::KEYS;
     const int key0 = min(split * share, limit), n_keys = min(share, limit - key0);
@@ -129,8 +142,21 @@ sdpa_decode_kernel(const DecodeParams p)
         const int s = j % NS;
         const uint32_t bytes = (uint32_t)min(Cfg::KEYS, n_keys - j * Cfg::KEYS) * Cfg::ROW;
         const uint32_t dst = sbase + (uint32_t)s * 2 * Cfg::TILE;
-        const size_t from = ((size_t)kvh * p.Sk + key0) * Cfg::ROW + (size_t)j * Cfg::TILE;
         ptx::mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
+        if constexpr (Cfg::WINDOW) {
+            const int c0 = key0 + j * Cfg::KEYS;
+            const uint32_t front = min((uint32_t)max(s_end - c0, 0) * Cfg::ROW, bytes);      // sinks of the stage
+            auto copy = [&](uint32_t at, int key, uint32_t n) {
+                if (n == 0) return;
+                const size_t from = ((size_t)kvh * p.Sk + key) * Cfg::ROW;
+                ptx::bulk_load(dst + at, static_cast<const char *>(p.k) + from, n, full + 8 * s);
+                ptx::bulk_load(dst + Cfg::TILE + at, static_cast<const char *>(p.v) + from, n, full + 8 * s);
+            };
+            copy(0, c0, front);
+            copy(front, max(c0, s_end) + skip, bytes - front);
+            return;
+        }
+        const size_t from = ((size_t)kvh * p.Sk + key0) * Cfg::ROW + (size_t)j * Cfg::TILE;
         ptx::bulk_load(dst, static_cast<const char *>(p.k) + from, bytes, full + 8 * s);
         ptx::bulk_load(dst + Cfg::TILE, static_cast<const char *>(p.v) + from, bytes, full + 8 * s);
     };
@@ -226,7 +252,10 @@ sdpa_decode_kernel(const DecodeParams p)
             for (int w = N; w < LPK; w <<= 1) sc[0] += __shfl_xor_sync(0xffffffffu, sc[0], w);
             float x = sc[0] * p.scale + mk;
             // also true for the rows of a stage that were never filled: whatever they hold is dropped here
-            if (key0 + j * Cfg::KEYS + my_kl >= my_lim) x = -INFINITY;
+            if constexpr (Cfg::WINDOW) {
+                const int c = key0 + j * Cfg::KEYS + my_kl, key = c < s_end ? c : c + skip, pos = off + my_row % p.Sq;
+                if (c >= limit || key >= last || key > pos || (key <= pos - p.win.window && key >= p.win.sinks)) x = -INFINITY;
+            } else if (key0 + j * Cfg::KEYS + my_kl >= my_lim) x = -INFINITY;
             float mn = fmaxf(m, x);
 #pragma unroll
             for (int w = 1; w < U; w <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));   // the row's other keys

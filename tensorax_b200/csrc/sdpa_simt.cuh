@@ -41,6 +41,7 @@ struct SimtParams {
     int out_f16;
     float scale;
     long long *prof;         // optional [32]: clock64 stamps of CTA (0,0,0), thread 0 (PROF instantiation only)
+    WindowRule win;          // WINDOW instantiations (window.cuh)
     const int *only_if = nullptr;   // optional: the launch does nothing unless x3_declines(only_if) (this kernel as the
                                     // stand-in behind a faster one that found it could not take the call)
 };
@@ -66,7 +67,7 @@ constexpr int SIMT_THREADS = 256;
 __device__ __forceinline__ float simt_load(const float *p) { return __ldg(p); }
 __device__ __forceinline__ float simt_load(const __half *p) { return __half2float(__ldg(p)); }
 
-template <typename T, int DVC, bool PROF = false>
+template <typename T, int DVC, bool PROF = false, bool WINDOW = false>
 __global__ void __launch_bounds__(SIMT_THREADS)
 sdpa_simt_kernel(const SimtParams p)
 {
@@ -110,7 +111,9 @@ sdpa_simt_kernel(const SimtParams p)
     int64_t key_end = p.Sk;
     key_end = p.kv_lens.limit((int)b, (int)key_end);
     const int64_t len_b = key_end;
-    if (p.causal) key_end = min(key_end, q0 + SIMT_BR);   // keys past the last row's diagonal
+    if (p.causal && !WINDOW) key_end = min(key_end, q0 + SIMT_BR);   // keys past the last row's diagonal
+    const int64_t pos0 = WINDOW ? q0 + p.win.offset((int)len_b, (int)p.Sq) : q0;
+    if (WINDOW) key_end = min(key_end, pos0 + SIMT_BR);
 
     // score phase mapping: 2 rows x 4 keys per thread
     const int sx = tid & 15, sy = tid >> 4;
@@ -126,6 +129,7 @@ sdpa_simt_kernel(const SimtParams p)
     for (int r = 0; r < 4; ++r) { m_run[r] = -FLT_MAX; l_run[r] = 0.f; }
 
     for (int64_t k0 = 0; k0 < key_end; k0 += SIMT_BC) {
+        if (WINDOW && k0 >= p.win.sinks && k0 + SIMT_BC <= pos0 - p.win.window + 1) continue;   // no row of the block sees the tile
         float acc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         for (int64_t d0 = 0; d0 < p.dk; d0 += SIMT_DKC) {
             __syncthreads();   // previous users of q_s / k_s / s_s are done
@@ -164,7 +168,9 @@ sdpa_simt_kernel(const SimtParams p)
                 const int64_t key = k0 + key_l;
                 float s = acc[r][c] * p.scale;
                 if (M && row < p.Sq && key < p.Sk) s += M[row * p.Sk + key];
-                const bool visible = key < len_b && (!p.causal || key <= row);
+                const int64_t pos = pos0 + row_l;
+                const bool visible = WINDOW ? key < len_b && key <= pos && (key > pos - p.win.window || key < p.win.sinks)
+                                            : key < len_b && (!p.causal || key <= row);
                 s_s[row_l][key_l] = visible ? s : -INFINITY;
             }
         }
@@ -199,7 +205,7 @@ sdpa_simt_kernel(const SimtParams p)
 #pragma unroll
             for (int c = 0; c < DVC; ++c) o[r][c] *= a;
         }
-        const int kmax = (int)min((int64_t)SIMT_BC, p.Sk - k0);
+        const int kmax = (int)min((int64_t)SIMT_BC, (WINDOW ? len_b : p.Sk) - k0);   // keys behind the last may hold anything
         for (int j = 0; j < kmax; ++j) {
             float vv[DVC];
 #pragma unroll
@@ -210,6 +216,7 @@ sdpa_simt_kernel(const SimtParams p)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float pj = s_s[warp * 4 + r][j];
+                if (WINDOW && pj == 0.f) continue;         // a key the row does not see may be anything, too
 #pragma unroll
                 for (int c = 0; c < DVC; ++c) o[r][c] = fmaf(pj, vv[c], o[r][c]);
             }

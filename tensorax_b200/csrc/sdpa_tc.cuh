@@ -37,6 +37,7 @@
 // `status` and the whole CTA drains and frees its tensor memory.
 #pragma once
 #include "ptx.cuh"
+#include "window.cuh"
 
 namespace txb {
 
@@ -55,6 +56,7 @@ struct TcParams {
     // sdpa_tc_pair_kernel only: the 1-D grid walks groups of `group` (batch, head) slabs; inside a group all
     // slabs' longest work items come first (n_pairs = 256-row query pairs per slab, BH = slabs)
     int group, n_pairs, BH;
+    WindowRule win;           // WINDOW instantiations (causal, keys outside a sliding window left out)
 };
 
 // Section profile (the counterpart of the reference's TX_TICK clock64 sections,
@@ -77,8 +79,9 @@ enum TcStatus : int {
 };
 
 template <int DK_, int DV_, int BN_, int NS_, bool P_TMEM_, bool PROF_ = false, int POLY_ = 0, int NSV_ = NS_,
-          bool LD_SPLIT_ = false, int QT_ = 0, bool Q_ALIAS_ = false>
+          bool LD_SPLIT_ = false, int QT_ = 0, bool Q_ALIAS_ = false, bool WINDOW_ = false>
 struct TcCfg {
+    static constexpr bool WINDOW = WINDOW_;   // sliding window with sinks (window.cuh)
     // Q_ALIAS: the Q panels that move to tensor memory are staged in the (still empty) K/V ring instead of
     // a region of their own; the producer starts the ring only after the copy.  Shared memory then holds
     // just the tail panels of Q, which is what lets d = 512 use 64-key tiles.
@@ -203,7 +206,10 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     kv_limit = p.kv_lens.limit(b, kv_limit);
     int kv_end = kv_limit;                                 // keys this query tile may see
     if (p.causal) kv_end = min(kv_end, q0 + BM);
-    const int n_tiles = (kv_end + BN - 1) / BN;
+    const int pos0 = Cfg::WINDOW ? q0 + p.win.offset(kv_limit, p.Sq) : q0;
+    const WindowWalk<BN> walk(p.win, kv_limit, pos0, BM);
+    const int n_tiles = Cfg::WINDOW ? walk.count() : (kv_end + BN - 1) / BN;
+    auto tile_of = [&](int j) { return Cfg::WINDOW ? walk.tile(j) : j; };
 
     if (tid == 0) {
         *abort_flag = 0;
@@ -282,7 +288,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                                 for (int pn = 0; pn < Cfg::KP; ++pn)
                                     ptx::tma_load_3d(k_s + s * Cfg::K_BYTES + pn * Cfg::KV_PANEL, &tm_k,
-                                                     k_full + 8 * s, pn * 64, jk * BN, kvh);
+                                                     k_full + 8 * s, pn * 64, tile_of(jk) * BN, kvh);
                             }
                             __syncwarp();
                             ++jk;
@@ -298,7 +304,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                                 for (int pn = 0; pn < Cfg::VP; ++pn)
                                     ptx::tma_load_3d(v_s + sv_ * Cfg::V_BYTES + pn * Cfg::KV_PANEL, &tm_v,
-                                                     v_full + 8 * sv_, dv0 + pn * 64, jv * BN, kvh);
+                                                     v_full + 8 * sv_, dv0 + pn * 64, tile_of(jv) * BN, kvh);
                             }
                             __syncwarp();
                             ++jv;
@@ -326,7 +332,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                         for (int pn = 0; pn < Cfg::KP; ++pn)
                             ptx::tma_load_3d(k_s + s * Cfg::K_BYTES + pn * Cfg::KV_PANEL, &tm_k,
-                                             k_full + 8 * s, pn * 64, j * BN, kvh);
+                                             k_full + 8 * s, pn * 64, tile_of(j) * BN, kvh);
                     }
                     __syncwarp();
                     const int sv_ = j % NSV;
@@ -340,7 +346,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 #pragma unroll
                         for (int pn = 0; pn < Cfg::VP; ++pn)
                             ptx::tma_load_3d(v_s + sv_ * Cfg::V_BYTES + pn * Cfg::KV_PANEL, &tm_v,
-                                             v_full + 8 * sv_, dv0 + pn * 64, j * BN, kvh);
+                                             v_full + 8 * sv_, dv0 + pn * 64, tile_of(j) * BN, kvh);
                     }
                     __syncwarp();
                 }
@@ -502,7 +508,7 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         tick_start();
         const long long t_begin = Cfg::PROF ? clock64() : 0;
         for (int j = 0; j < n_tiles && ok; ++j) {
-            const int kv0 = j * BN;
+            const int kv0 = tile_of(j) * BN;
             tick(0);
             ok = wait_all(s_full, (uint32_t)j & 1u);
             tick(SEC_SM_WAIT_S);
@@ -516,8 +522,13 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             arrive_warp(s_free);
             tick(SEC_SM_LOAD_S);
 
-            const bool need_mask = (j * BN + BN > kv_limit) || (p.causal && (j * BN + BN - 1 > q0));
-            if (need_mask) {
+            const bool need_mask = Cfg::WINDOW ? window_edge(p.win, kv_limit, pos0, BM, kv0, BN)
+                                               : (j * BN + BN > kv_limit) || (p.causal && (j * BN + BN - 1 > q0));
+            if (Cfg::WINDOW && need_mask) {
+                const WindowColumns seen(p.win, kv_limit, pos0 + r, kv0);
+#pragma unroll
+                for (int i = 0; i < BN; ++i) sv[i] = keep_if_seen(sv[i], i, seen);
+            } else if (need_mask) {
                 // visible keys of this row are a prefix of the tile: columns [0, lim)
                 const int lim = min(kv_limit - kv0, p.causal ? row - kv0 + 1 : BN);
 #pragma unroll
@@ -586,6 +597,12 @@ sdpa_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     ptx::tmem_wait_st();
                 }
                 tick(SEC_SM_RESCALE);
+            }
+            if (Cfg::WINDOW && kv0 + BN > kv_limit) {     // what lies behind the sequence's last key
+                ok = wait_all(v_full + 8 * (j % NSV), (uint32_t)(j / NSV) & 1u);
+                if (!ok) break;
+                zero_stage_rows<BN, 32 * Cfg::SOFTMAX_WARPS>(smem + Cfg::OFF_V + (j % NSV) * Cfg::V_BYTES, Cfg::VP, kv_limit - kv0, r);
+                ptx::fence_proxy_async_smem();
             }
             if constexpr (Cfg::P_TMEM) {
                 ptx::tmem_st_cols<BN / 2>(t_p, pk);

@@ -50,8 +50,10 @@ enum PairSection : int {
 // FAULT_TEST: the instantiation behind tx_selftest_wait_timeout -- every wait gives up after 2 ms instead of 2 s and
 //       the producer leaves out the K tile TcParams::skip_k_tile names, so that the give-up path can be exercised
 //       on a GPU without faulting or hanging anything.
-template <int D_, int BN_, int NS_, int POLY_, bool P_ALIAS_, bool PROF_ = false, bool FAULT_TEST_ = false>
+template <int D_, int BN_, int NS_, int POLY_, bool P_ALIAS_, bool PROF_ = false, bool FAULT_TEST_ = false,
+          bool WINDOW_ = false>
 struct PairCfg {
+    static constexpr bool WINDOW = WINDOW_;   // sliding window with sinks (window.cuh)
     static constexpr int D = D_, BN = BN_, NS = NS_, POLY = POLY_;
     static constexpr bool P_ALIAS = P_ALIAS_, PROF = PROF_, FAULT_TEST = FAULT_TEST_;
     static constexpr uint64_t WAIT_NS = FAULT_TEST_ ? 2000000ull : kWaitLimitNs;
@@ -143,7 +145,13 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool live1 = q0 + BM < p.Sq;
     const int kv_end0 = p.causal ? min(kv_limit, q0 + BM) : kv_limit;
     const int kv_end1 = live1 ? (p.causal ? min(kv_limit, q0 + 2 * BM) : kv_limit) : 0;
-    const int n0 = (kv_end0 + BN - 1) / BN, n1 = (kv_end1 + BN - 1) / BN;
+    // With a window both tiles walk one list, that of all their rows: the second one's first entry may be masked as a
+    // whole (one tile of window / BN + 2), which costs less than two rings.
+    const int off = Cfg::WINDOW ? p.win.offset(kv_limit, p.Sq) : 0;
+    const WindowWalk<BN> walk(p.win, kv_limit, off + q0, live1 ? 2 * BM : BM);
+    const int n0 = Cfg::WINDOW ? walk.count_below(off + q0 + BM) : (kv_end0 + BN - 1) / BN;
+    const int n1 = Cfg::WINDOW ? (live1 ? walk.count() : 0) : (kv_end1 + BN - 1) / BN;
+    auto tile_of = [&](int j) { return Cfg::WINDOW ? walk.tile(j) : j; };
     const int n_max = max(n0, n1);
 
     // Warp 0 sets the barriers up and sends the first loads (both Q tiles, K and V of key tile 0) on their way
@@ -184,7 +192,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                     ptx::mbar_arrive_expect_tx(k_full, Cfg::K_BYTES);
 #pragma unroll
                     for (int pn = 0; pn < Cfg::KP; ++pn)
-                        ptx::tma_load_3d(k_s + pn * Cfg::KV_PANEL, &tm_k, k_full, pn * 64, 0, kvh);
+                        ptx::tma_load_3d(k_s + pn * Cfg::KV_PANEL, &tm_k, k_full, pn * 64, tile_of(0) * BN, kvh);
                 }
                 if (n1 > 0) {
                     ptx::mbar_arrive_expect_tx(q_full + 8, Cfg::Q_TILE_BYTES);
@@ -196,7 +204,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 ptx::mbar_arrive_expect_tx(v_full, Cfg::V_BYTES);
 #pragma unroll
                 for (int pn = 0; pn < Cfg::KP; ++pn)
-                    ptx::tma_load_3d(v_s + pn * Cfg::KV_PANEL, &tm_v, v_full, pn * 64, 0, kvh);
+                    ptx::tma_load_3d(v_s + pn * Cfg::KV_PANEL, &tm_v, v_full, pn * 64, tile_of(0) * BN, kvh);
             }
             // an earlier CTA of the launch may already have given up (asked after the loads are out: the answer
             // takes a trip to global memory; the loads land during the teardown's grace period)
@@ -237,7 +245,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
                     for (int pn = 0; pn < Cfg::KP; ++pn)
                         ptx::tma_load_3d(k_s + s * Cfg::K_BYTES + pn * Cfg::KV_PANEL, &tm_k, k_full + 8 * s,
-                                         pn * 64, j * BN, kvh);
+                                         pn * 64, tile_of(j) * BN, kvh);
                 }
                 __syncwarp();
                 ok = ptx::mbar_wait(v_empty + 8 * s, ph ^ 1u, abort_flag, Cfg::WAIT_NS);
@@ -247,7 +255,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
 #pragma unroll
                     for (int pn = 0; pn < Cfg::KP; ++pn)
                         ptx::tma_load_3d(v_s + s * Cfg::V_BYTES + pn * Cfg::KV_PANEL, &tm_v, v_full + 8 * s,
-                                         pn * 64, j * BN, kvh);
+                                         pn * 64, tile_of(j) * BN, kvh);
                 }
                 __syncwarp();
             }
@@ -397,7 +405,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         tick_start();
         const long long t_begin = Cfg::PROF ? clock64() : 0;
         for (int j = 0; j < nt && ok; ++j) {
-            const int kv0 = j * BN;
+            const int kv0 = tile_of(j) * BN;
             tick(0);
             ok = ptx::mbar_wait(my_s_full, (uint32_t)j & 1u, abort_flag, Cfg::WAIT_NS);
             tick(PSEC_SM_WAIT_S);
@@ -413,8 +421,13 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             ptx::reg_fence_cols<BN>(sv);
             if constexpr (!Cfg::P_ALIAS) arrive_warp(my_s_free);   // S belongs to the MMA warp again
             tick(PSEC_SM_LOAD_S);
-            const bool need_mask = (kv0 + BN > kv_limit) || (p.causal && (kv0 + BN - 1 > q0t));
-            if (need_mask) {
+            const bool need_mask = Cfg::WINDOW ? window_edge(p.win, kv_limit, off + q0t, BM, kv0, BN)
+                                               : (kv0 + BN > kv_limit) || (p.causal && (kv0 + BN - 1 > q0t));
+            if (Cfg::WINDOW && need_mask) {
+                const WindowColumns seen(p.win, kv_limit, off + row, kv0);
+#pragma unroll
+                for (int i = 0; i < BN; ++i) sv[i] = keep_if_seen(sv[i], i, seen);
+            } else if (need_mask) {
                 // visible keys of this row are a prefix of the tile: columns [0, lim)
                 const int lim = min(kv_limit - kv0, p.causal ? row - kv0 + 1 : BN);
 #pragma unroll
@@ -474,6 +487,13 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 }
             }
             tick(PSEC_SM_WAIT_PV);
+            if (Cfg::WINDOW && kv0 + BN > kv_limit && (t == 0 || j >= n0)) {
+                // what lies behind the sequence's last key; query tile 0's PV comes before tile 1's, so its warps do it for both
+                ok = ptx::mbar_wait(v_full + 8 * (j % NS), (uint32_t)(j / NS) & 1u, abort_flag, Cfg::WAIT_NS);
+                if (!ok) break;
+                zero_stage_rows<BN, 128>(smem + Cfg::OFF_V + (j % NS) * Cfg::V_BYTES, Cfg::KP, kv_limit - kv0, r);
+                ptx::fence_proxy_async_smem();
+            }
             ptx::tmem_st_cols<BN / 2>(t_p, pk);
             ptx::tmem_wait_st();
             arrive_warp(my_p_full);
@@ -485,7 +505,9 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if constexpr (Cfg::PROF) { if (prof_lane) p.prof[(t ? 32 : 0) + PSEC_SM_EPI_PV] = clock64() - t_loop_end; }
             if (ok) {
                 ptx::tc_fence_after_sync();
-                const float inv_l = 1.0f / l;    // l == 0 (no visible key) -> inf -> NaN rows, as the reference
+                // l == 0 (no visible key) -> inf -> NaN rows, as the reference; with a window a row may stay without one beside
+                // others, and the polynomial's 2^(-inf) is not quite 0
+                const float inv_l = Cfg::WINDOW && m_used == -1.0e30f ? __int_as_float(0x7fc00000) : 1.0f / l;
                 if (p.lse && row < p.Sq) p.lse[(size_t)bh * p.Sq + row] = m_used + __log2f(l);
                 // O leaves through shared memory and one bulk tensor store per 128-byte-wide chunk of this warp's
                 // 32 rows: a thread owns a row, so direct stores would put 32 rows' 16-byte pieces into every

@@ -40,8 +40,9 @@ namespace txb {
 
 constexpr int X3_TILE = 64;      // keys per tile, each tile of K and V with a factor of its own; the split pass's CTAs
 
-template <int D_, int NS_, bool MASK_ = false>
+template <int D_, int NS_, bool MASK_ = false, bool WINDOW_ = false>
 struct X3Cfg {
+    static constexpr bool WINDOW = WINDOW_;                // sliding window with sinks (window.cuh)
     static constexpr int D = D_, NS = NS_;                 // D: 64 or 128, at least d_k and d_v
     static constexpr bool MASK = MASK_;
     // Stages of the mask tile, as many as shared memory has room for: the mask comes from memory, 32 KB a tile, and with two
@@ -107,6 +108,7 @@ struct X3Params {
     float scale;              // 1/sqrt(d_k)
     float scale_log2;         // scale * log2(e)
     int group, n_tiles_q, BH; // work-item order, as in sdpa_tc_pair_kernel (query tiles in place of pairs)
+    WindowRule win;           // WINDOW instantiations
 };
 
 template <class Cfg>
@@ -154,15 +156,18 @@ sdpa_tc_x3_kernel(const __grid_constant__ CUtensorMap tm_qh, const __grid_consta
     int kv_limit = p.Sk;                                         // keys any row of this batch may see
     kv_limit = p.kv_lens.limit(b, kv_limit);
     const int kv_end = p.causal ? min(kv_limit, q0 + BM) : kv_limit;
-    const int nt = (kv_end + BN - 1) / BN;
+    const int pos0 = Cfg::WINDOW ? q0 + p.win.offset(kv_limit, p.Sq) : q0;
+    const WindowWalk<BN> walk(p.win, kv_limit, pos0, BM);
+    const int nt = Cfg::WINDOW ? walk.count() : (kv_end + BN - 1) / BN;
+    auto tile_of = [&](int j) { return Cfg::WINDOW ? walk.tile(j) : j; };
 
     auto load_kv = [&](uint32_t dst, const CUtensorMap *hi, const CUtensorMap *lo, uint32_t bar, int j, int panels) {
         ptx::mbar_arrive_expect_tx(bar, 2 * Cfg::KV_PANEL * (uint32_t)panels);
 #pragma unroll
         for (int pn = 0; pn < Cfg::KP; ++pn) {
             if (pn >= panels) break;
-            ptx::tma_load_3d(dst + pn * Cfg::KV_PANEL, hi, bar, pn * 64, j * BN, kvh);
-            ptx::tma_load_3d(dst + Cfg::KV_BYTES + pn * Cfg::KV_PANEL, lo, bar, pn * 64, j * BN, kvh);
+            ptx::tma_load_3d(dst + pn * Cfg::KV_PANEL, hi, bar, pn * 64, tile_of(j) * BN, kvh);
+            ptx::tma_load_3d(dst + Cfg::KV_BYTES + pn * Cfg::KV_PANEL, lo, bar, pn * 64, tile_of(j) * BN, kvh);
         }
     };
 
@@ -385,7 +390,7 @@ sdpa_tc_x3_kernel(const __grid_constant__ CUtensorMap tm_qh, const __grid_consta
         if (run && warp == 4) {                          // how far V's keys lie apart, while the first tiles are on their way
             int most = 0, least = 255;
             for (int j = lane; j < nt; j += 32) {
-                const int f = p.vr[f0 + j];
+                const int f = p.vr[f0 + tile_of(j)];
                 most = max(most, f & 255);
                 least = min(least, f >> 8);
             }
@@ -399,9 +404,9 @@ sdpa_tc_x3_kernel(const __grid_constant__ CUtensorMap tm_qh, const __grid_consta
             if (lane == 0) ptx::mbar_arrive(bar);
         };
         for (int j = 0; j < nt && ok; ++j) {
-            const int kv0 = j * BN;
+            const int kv0 = tile_of(j) * BN;
             // not 0, however small the factors: -inf * 0 would make a NaN of a key that is not seen
-            const float tile_scale = fmaxf(row_scale * p.kf[f0 + j], FLT_MIN), scale = Cfg::MASK ? kLog2e : tile_scale;
+            const float tile_scale = fmaxf(row_scale * p.kf[f0 + tile_of(j)], FLT_MIN), scale = Cfg::MASK ? kLog2e : tile_scale;
             ok = ptx::mbar_wait(s_full, (uint32_t)j & 1u, abort_flag);
             if (!ok) break;
             ptx::tc_fence_after_sync();
@@ -427,8 +432,13 @@ sdpa_tc_x3_kernel(const __grid_constant__ CUtensorMap tm_qh, const __grid_consta
                 __syncwarp();
                 if (lane == 0) ptx::mbar_arrive(mask_empty + 8 * sm_);
             }
-            const bool need_mask = (kv0 + BN > kv_limit) || (p.causal && (kv0 + BN - 1 > q0));
-            if (need_mask) {
+            const bool need_mask = Cfg::WINDOW ? window_edge(p.win, kv_limit, pos0, BM, kv0, BN)
+                                               : (kv0 + BN > kv_limit) || (p.causal && (kv0 + BN - 1 > q0));
+            if (Cfg::WINDOW && need_mask) {
+                const WindowColumns seen(p.win, kv_limit, pos0 + r, kv0);
+#pragma unroll
+                for (int i = 0; i < BN; ++i) sv[i] = keep_if_seen(sv[i], i, seen);
+            } else if (need_mask) {
                 // visible keys of this row are a prefix of the tile: columns [0, lim)
                 const int lim = min(kv_limit - kv0, p.causal ? row - kv0 + 1 : BN);
 #pragma unroll
@@ -510,7 +520,7 @@ sdpa_tc_x3_kernel(const __grid_constant__ CUtensorMap tm_qh, const __grid_consta
         const int f0 = kvh * ((p.Sk + BN - 1) / BN);
         for (int j = 0; j < nt && ok; ++j) {
             const int a = j & 1;
-            const float beta = p.vf[f0 + j];             // asked for before the waits
+            const float beta = p.vf[f0 + tile_of(j)];             // asked for before the waits
             ok = ptx::mbar_wait(alpha_full + 8 * (j & 3), (uint32_t)(j >> 2) & 1u, abort_flag);
             if (!ok) break;
             const float alpha = alpha_s[(j & 3) * BM + r];

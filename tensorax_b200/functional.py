@@ -152,6 +152,37 @@ def scaled_dot_product_attention_ex(query: Tensor, key: Tensor, value: Tensor,
     return _result(c)
 
 
+def scaled_dot_product_attention_window(query: Tensor, key: Tensor, value: Tensor, window: int, sinks: int = 0,
+                                        kv_lens: Optional[Sequence[int]] = None, align: str = "start",
+                                        out_dtype: str = "float32", grad_dtype: str = "float32",
+                                        sync: bool = True) -> Tensor:
+    """No reference counterpart.  Causal attention with a sliding window: row i at position p sees key j iff j <= p,
+    j < kv_lens[b], and j > p - window or j < sinks (first keys that stay visible).  ``align="start"``: p = i;
+    ``align="end"``: the rows are the last ones of their sequence, p = kv_lens[b] - Sq + i (a decoding step, or a chunk of
+    a long prompt).  K/V may have fewer heads than Q; float16 and float32.  A row that sees no key is NaN.  Differentiable
+    for float16 with d in {64, 128, 256}; ``grad_dtype="float16"`` leaves the gradients in float16."""
+    _check(query, key, value, None, _MSG4D)
+    if grad_dtype not in ("float32", "float16"):
+        raise ValueError("grad_dtype must be 'float32' or 'float16'")
+    if not _C:
+        raise RuntimeError("C++ backend not available.")
+    q, k, v = query._c_tensor, key._c_tensor, value._c_tensor
+    needs_grad = query.requires_grad or key.requires_grad or value.requires_grad
+    if not needs_grad:
+        return _result(_C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens,
+                                                              out_dtype=out_dtype, sync=sync))
+    grad_fn = ("scaled_dot_product_attention", query, key, value, None)
+    if not _C.sdpa_backward_supported(q, k, v, None):
+        return _result(_C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens,
+                                                              out_dtype=out_dtype, sync=sync), True, grad_fn)
+    c, lse = _C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens, out_dtype=out_dtype,
+                                                    want_lse=True, sync=sync)
+    out = _result(c, True, grad_fn)
+    out._saved = {"lse": lse, "causal": True, "kv_lens": None if kv_lens is None else list(kv_lens),
+                  "window": _C.window_desc(window, sinks, align), "grad_dtype": grad_dtype}
+    return out
+
+
 # ------------------------------------------------------------------ quantised K/V cache (no reference counterpart)
 def _check_cache(cache, *tensors):
     if not _C:

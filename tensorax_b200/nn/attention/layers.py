@@ -47,11 +47,24 @@ class GroupedQueryAttention:
         return F.scaled_dot_product_attention(query, key, value, mask)
 
     def forward_bhsd(self, query: Tensor, key: Tensor, value: Tensor, mask: Tensor = None,
-                     causal: bool = False, kv_lens=None) -> Tensor:
-        """query [B, num_heads, S, d]; key/value [B, num_kv_heads, S, d]."""
+                     causal: bool = False, kv_lens=None, window=None, sinks: int = 0, align: str = "start") -> Tensor:
+        """query [B, num_heads, S, d]; key/value [B, num_kv_heads, S, d].  ``window`` (with ``sinks`` and ``align``): causal
+        attention to the last keys only, ``F.scaled_dot_product_attention_window``."""
         if query.shape[1] != self.num_heads or key.shape[1] != self.num_kv_heads:
             raise ValueError("forward_bhsd: head counts do not match the layer")
+        if window is not None:
+            if mask is not None:
+                raise ValueError("forward_bhsd: a window takes no dense mask")
+            return F.scaled_dot_product_attention_window(query, key, value, window, sinks, kv_lens=kv_lens, align=align)
         return F.scaled_dot_product_attention_ex(query, key, value, mask, causal=causal, kv_lens=kv_lens)
+
+    def forward_cached(self, query: Tensor, cache, page_table, kv_lens, q_lens=None, tree=None, window=None,
+                       sinks: int = 0, out_dtype: str = "float32") -> Tensor:
+        """query [B, num_heads, T, d] of each sequence's last tokens over a ``QuantizedKVCache`` of num_kv_heads heads
+        (``F.kv_cache_attention``)."""
+        if query.shape[1] != self.num_heads or cache.num_kv_heads != self.num_kv_heads:
+            raise ValueError("forward_cached: head counts do not match the layer")
+        return F.kv_cache_attention(query, cache, page_table, kv_lens, q_lens, tree, window, sinks, out_dtype)
 
     def __call__(self, query: Tensor, key: Tensor, value: Tensor, mask: Tensor = None) -> Tensor:
         return self.forward(query, key, value, mask)

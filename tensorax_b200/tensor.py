@@ -160,7 +160,8 @@ class Tensor:
             raise RuntimeError("gradient accumulation is not available in tensorax_b200: clear .grad of the inputs first")
         dq, dk, dv = _C.scaled_dot_product_attention_backward(
             query._c_tensor, key._c_tensor, value._c_tensor, self._c_tensor, saved["lse"], g._c_tensor,
-            causal=saved["causal"], kv_lens=saved["kv_lens"])
+            causal=saved["causal"], kv_lens=saved["kv_lens"], window=saved.get("window"),
+            grad_dtype=saved.get("grad_dtype", "float32"))
         for t, c in ((query, dq), (key, dk), (value, dv)):
             if t.requires_grad:
                 t.backward(Tensor._wrap(c))

@@ -12,7 +12,7 @@ def quantise(x, fmt):
     x = np.where(fine[..., None], x, np.float32(0))
     amax = np.abs(x).max(-1)
     if fmt == "int8":
-        scale = np.maximum(amax / np.float32(127), np.float32(2.0 ** -126)).astype(np.float32)
+        scale = np.maximum(amax * (np.float32(1) / np.float32(127)), np.float32(2.0 ** -126)).astype(np.float32)
         codes = np.clip(np.rint(x / scale[..., None]), -127, 127).astype(np.int8)
     else:
         m, e = np.frexp(amax.astype(np.float64))
