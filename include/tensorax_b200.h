@@ -40,7 +40,7 @@ enum {
                               12/13/14 linear-kernel producer / MMA / split warps, 22/23/24 backward
                               producer / MMA / row warps, 32/34 decoding-kernel producer / row warps,
                               42/43/44 layer-GEMM producer / MMA / summing warps; 51 is a page or a row that a K/V cache
-                              call names and that does not exist */
+                              call names and that does not exist, 54 its attention's wait for keys */
     TX_ERR_UNSUPPORTED = 5
 };
 
@@ -334,7 +334,7 @@ TX_API int tx_sdpa_window_backward(const tx_sdpa_bwd_desc *desc, const tx_window
  *      and attention gives NaN to the rows that see it and to no others.
  *      Token `pos` of sequence b lies in page page_table[b][pos / page_size], place pos % page_size.  Pages may be shared
  *      between sequences as long as nobody writes them; two rows of one call that are written to one place race.
- *      All pointers are device pointers (k, v, q, out and the codes 16-byte aligned), everything is asynchronous on `stream`
+ *      All pointers are device pointers (k, v, q, out, the codes and the scales 16-byte aligned), everything is asynchronous on `stream`
  *      and captures into graphs; no call allocates.  A token without a page (a position beyond the table, an entry outside
  *      [0, pages)) is left out, never followed, and reported: tx_sdpa_finish then returns TX_ERR_KERNEL (stage code 51), and
  *      attention rows of the sequences concerned are NaN. */

@@ -29,17 +29,17 @@ int pages_of(const char *who, const tx_kv_cache &c, const int32_t *table, int64_
              txb::KvPages *out)
 {
     if (!c.k || !c.v || !c.k_scale || !c.v_scale || !table) return fail(TX_ERR_INVALID, "%s: null pointer", who);
-    if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 4) || !aligned(c.v_scale, 4) || !aligned(table, 4))
-        return fail(TX_ERR_INVALID, "%s: the cache's codes must be 16-byte aligned, scales and page table 4-byte", who);
+    if (!aligned(c.k, 16) || !aligned(c.v, 16) || !aligned(c.k_scale, 16) || !aligned(c.v_scale, 16) || !aligned(table, 4))
+        return fail(TX_ERR_INVALID, "%s: the cache's codes and scales must be 16-byte aligned, the page table 4-byte", who);
     if (c.pages <= 0 || c.kv_heads <= 0 || batch <= 0 || table_len <= 0) return fail(TX_ERR_INVALID, "%s: every dimension must be positive", who);
     if (c.d != 64 && c.d != 128 && c.d != 256) return fail(TX_ERR_UNSUPPORTED, "%s: head dim must be 64, 128 or 256", who);
     if (c.page_size < 16 || c.page_size > 65536 || (c.page_size & (c.page_size - 1)))
         return fail(TX_ERR_INVALID, "%s: page_size must be a power of two from 16 to 65536", who);
     if (c.format != TX_KV_E4M3 && c.format != TX_KV_INT8) return fail(TX_ERR_INVALID, "%s: format must be TX_KV_E4M3 or TX_KV_INT8", who);
     if (dtype != TX_DTYPE_F32 && dtype != TX_DTYPE_F16) return fail(TX_ERR_INVALID, "%s: dtype must be float32 or float16", who);
-    // positions and (batch, head) numbers are 32-bit in the kernels; row numbers and byte offsets are 64-bit
+    // positions, rows of the cache and its 128-byte lines are 32-bit numbers, byte offsets 64-bit
     if (c.pages > 0x7fffffffLL || c.kv_heads > 65535 || batch > 0xffffffLL || batch * c.kv_heads > 0x3fffffffLL || table_len > 0x7fffffffLL ||
-        table_len * c.page_size > 0x7fffffffLL)
+        table_len * c.page_size > 0x7fffffffLL || c.pages * c.kv_heads > 0x7fffffffLL / (c.page_size * (c.d / 64)))
         return fail(TX_ERR_UNSUPPORTED, "%s: dimension too large", who);
     out->k = static_cast<uint8_t *>(c.k); out->v = static_cast<uint8_t *>(c.v);
     out->ks = c.k_scale; out->vs = c.v_scale;
@@ -140,7 +140,11 @@ int launch_attention_t(txb::KvAttnParams p, const tx_kv_attention_desc *d)
     cfg.stream = static_cast<cudaStream_t>(d->stream);
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    TX_CUDA(cudaLaunchKernelEx(&cfg, txb::kv_attention_kernel<Cfg>, p));
+    CUtensorMap tk, tv;
+    const int64_t cache_rows = d->cache.pages * d->cache.kv_heads * d->cache.page_size;
+    if (int rc = txb::api::map_of_codes(&tk, d->cache.k, cache_rows, d->cache.d)) return rc;
+    if (int rc = txb::api::map_of_codes(&tv, d->cache.v, cache_rows, d->cache.d)) return rc;
+    TX_CUDA(cudaLaunchKernelEx(&cfg, txb::kv_attention_kernel<Cfg>, tk, tv, p));
     txb::api::launched();
     return TX_OK;
 }
@@ -149,13 +153,18 @@ template <typename T, int FMT, int D>
 int launch_attention(const txb::KvAttnParams &p, const tx_kv_attention_desc *d)
 {
     const int64_t rows = (int64_t)p.group * p.tokens;
+    // Rows of a part: eight at a time up to 32 (16 at d = 256), as registers hold them.  Steps of 32 keys where registers allow
+    // (B16 Hkv8, 8192 keys, d128: four rows 67.6 us with 32 keys a step and three CTAs an SM, 69.7 with 16 and four; sixteen
+    // rows 71.7 and 101; 32 rows a head at 256 in all 352 and 463).
+    constexpr bool F32 = sizeof(T) == 4;
     if constexpr (D == 256) {
-        if (rows <= 16) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 1, 4, 16, 3, sizeof(T) == 4 ? 1 : 2>>(p, d);
-        return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 2, 2, 16, 4, 2>>(p, d);
+        if (rows <= 8) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 1, 4, 16, 3, F32 ? 1 : 2>>(p, d);
+        return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 2, 4, 16, 3, F32 ? 1 : 2>>(p, d);
     } else {
-        if (rows <= 16) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 1, 4, 32, 3, 2>>(p, d);
-        if (rows <= 32) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 2, 2, 32, 4, 2>>(p, d);
-        return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 4, 2, 32, 4, 1>>(p, d);
+        constexpr int NS1 = D == 64 ? 4 : F32 ? 3 : 2, NS = D == 64 ? 4 : 3;
+        if (rows <= 8) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 1, 4, 32, NS1, F32 ? 2 : 3>>(p, d);
+        if (rows <= 16) return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 2, 4, F32 ? 16 : 32, F32 ? 4 : NS, 2>>(p, d);
+        return launch_attention_t<txb::KvAttnCfg<T, FMT, D, 4, 4, F32 ? 16 : 32, F32 ? 4 : NS, 2>>(p, d);
     }
 }
 

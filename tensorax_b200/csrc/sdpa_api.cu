@@ -163,7 +163,7 @@ int get_encode_fn(EncodeTiledFn *fn)
     return TX_OK;
 }
 
-// fp16 (or fp32: elem_bytes 4) tensor [slabs, rows, d] -> 3-D map (d, rows, slabs); box = 128 bytes of a row x
+// fp16 (or fp32: elem_bytes 4, bytes: 1) tensor [slabs, rows, d] -> 3-D map (d, rows, slabs); box = 128 bytes of a row x
 // box_rows, 128B swizzle.
 // A map is a pure function of (base, slabs, rows, d, box_rows): the last few are kept per host thread, so a
 // caller that runs the same buffers again (a decoding loop, a benchmark) does not pay the driver's encode
@@ -203,7 +203,8 @@ int make_map(CUtensorMap *m, const void *base, int64_t slabs, int64_t rows, int6
     cuuint64_t strides[2] = {(cuuint64_t)d * eb, (cuuint64_t)rows * (cuuint64_t)d * eb};
     cuuint32_t box[3] = {(cuuint32_t)(128 / elem_bytes), (cuuint32_t)box_rows, 1};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(m, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+    CUresult r = enc(m, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : elem_bytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                                  : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
                      const_cast<void *>(base), dims, strides,
                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1463,6 +1464,7 @@ int ensure_device() { return ::ensure_device(); }
 int status_word(int **out) { return ::status_word(out); }
 int sm_count(int *n) { return ::sm_count(n); }
 int current_device(int *dev) { return ::current_device(dev); }
+int map_of_codes(CUtensorMap *m, const void *base, int64_t rows, int64_t d) { return make_map(m, base, 1, rows * d / 128, 128, (int)(d / 8), 1); }
 void launched() { g_launches++; }
 
 }  // namespace api
