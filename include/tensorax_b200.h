@@ -40,7 +40,8 @@ enum {
                               12/13/14 linear-kernel producer / MMA / split warps, 22/23/24 backward
                               producer / MMA / row warps, 32/34 decoding-kernel producer / row warps,
                               42/43/44 layer-GEMM producer / MMA / summing warps; 51 is a page or a row that a K/V cache
-                              call names and that does not exist, 54 its attention's wait for keys */
+                              call names and that does not exist, 54 its attention's wait for keys,
+                              55/56/57 MMA / converter / softmax warps of its attention of many rows */
     TX_ERR_UNSUPPORTED = 5
 };
 

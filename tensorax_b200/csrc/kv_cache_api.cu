@@ -9,6 +9,7 @@
 
 #include "api_internal.h"
 #include "kv_attention.cuh"
+#include "kv_attention_tc.cuh"
 #include "kv_cache.cuh"
 
 namespace {
@@ -115,44 +116,76 @@ int allow_launch(int smem)
     return TX_OK;
 }
 
+// CTAs of a cluster that share the keys of an item: as many as one wave holds, as long as each has a tile of KT of the most
+// keys that the call can see
+int splits_of(const tx_kv_attention_desc *d, int64_t items, int64_t places, int most, int kt)
+{
+    int64_t keys = d->table_len * d->cache.page_size;
+    if (d->window > 0) keys = std::min(keys, d->window + d->sinks + d->tokens);
+    int splits = 1;
+    while (splits < most && items * splits * 2 <= places && (int64_t)splits * kt < keys) splits *= 2;
+    return splits;
+}
+
+template <class... Params, class... Args>
+int launch_cluster(void (*kernel)(Params...), int64_t ctas, int cluster, int threads, size_t smem, void *stream, const Args &...args)
+{
+    if (ctas > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "K/V cache attention: more than 2^31 work items");
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    TX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    txb::api::launched();
+    return TX_OK;
+}
+
 template <class Cfg>
 int launch_attention_t(txb::KvAttnParams p, const tx_kv_attention_desc *d)
 {
     const int64_t rows = (int64_t)p.group * p.tokens;
     p.row_parts = (int)((rows + Cfg::MR - 1) / Cfg::MR);
     const int64_t items = d->batch * d->cache.kv_heads * p.row_parts;
-    if (items * Cfg::MAX_SPLITS > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "K/V cache attention: more than 2^31 work items");
     int sms = 0;
     if (int rc = txb::api::sm_count(&sms)) return rc;
-    // CTAs per item: as many as one wave holds, as long as each has a stage of the most keys that the call can see
-    int64_t keys = d->table_len * d->cache.page_size;
-    if (d->window > 0) keys = std::min(keys, d->window + d->sinks + d->tokens);
-    int splits = 1;
-    while (splits < Cfg::MAX_SPLITS && items * splits * 2 <= (int64_t)Cfg::CTAS_PER_SM * sms && (int64_t)splits * Cfg::KT < keys) splits *= 2;
+    const int splits = splits_of(d, items, (int64_t)Cfg::CTAS_PER_SM * sms, Cfg::MAX_SPLITS, Cfg::KT);
     if (int rc = allow_launch<txb::kv_attention_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)splits; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(items * splits));
-    cfg.blockDim = dim3(Cfg::THREADS);
-    cfg.dynamicSmemBytes = Cfg::SMEM;
-    cfg.stream = static_cast<cudaStream_t>(d->stream);
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
     CUtensorMap tk, tv;
     const int64_t cache_rows = d->cache.pages * d->cache.kv_heads * d->cache.page_size;
     if (int rc = txb::api::map_of_codes(&tk, d->cache.k, cache_rows, d->cache.d)) return rc;
     if (int rc = txb::api::map_of_codes(&tv, d->cache.v, cache_rows, d->cache.d)) return rc;
-    TX_CUDA(cudaLaunchKernelEx(&cfg, txb::kv_attention_kernel<Cfg>, tk, tv, p));
-    txb::api::launched();
-    return TX_OK;
+    return launch_cluster(txb::kv_attention_kernel<Cfg>, items * splits, splits, Cfg::THREADS, Cfg::SMEM, d->stream, tk, tv, p);
 }
+
+template <class Cfg>
+int launch_attention_tc(txb::KvAttnParams p, const tx_kv_attention_desc *d)
+{
+    const int64_t rows = (int64_t)p.group * p.tokens;
+    p.row_parts = (int)((rows + Cfg::MR - 1) / Cfg::MR);
+    const int64_t items = d->batch * d->cache.kv_heads * p.row_parts;
+    int sms = 0;
+    if (int rc = txb::api::sm_count(&sms)) return rc;
+    const int splits = splits_of(d, items, sms, Cfg::MAX_SPLITS, Cfg::BN);
+    if (int rc = allow_launch<txb::kv_attention_tc_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
+    return launch_cluster(txb::kv_attention_tc_kernel<Cfg>, items * splits, splits, Cfg::THREADS, Cfg::SMEM, d->stream, p);
+}
+
+// More query rows per K/V head than this: the tcgen05 kernel, whose CTA takes 256 at once.  B8 Hkv8 d128, 8192 keys: 32 rows a head
+// 57 us here and 96 there, 64 rows 94 and 98, 128 rows 162 and 100; B1, 2000 keys: 64 rows 33 and 29.
+constexpr int kTcRows = 64;
 
 template <typename T, int FMT, int D>
 int launch_attention(const txb::KvAttnParams &p, const tx_kv_attention_desc *d)
 {
     const int64_t rows = (int64_t)p.group * p.tokens;
+    if constexpr (sizeof(T) == 2 && D <= 128)
+        if (rows > kTcRows) return launch_attention_tc<txb::KvTcCfg<FMT, D, D == 64 ? 0x0303 : 0x0003>>(p, d);
     // Rows of a part: eight at a time up to 32 (16 at d = 256), as registers hold them.  Steps of 32 keys where registers allow
     // (B16 Hkv8, 8192 keys, d128: four rows 67.6 us with 32 keys a step and three CTAs an SM, 69.7 with 16 and four; sixteen
     // rows 71.7 and 101; 32 rows a head at 256 in all 352 and 463).

@@ -116,8 +116,9 @@ def test_what_does_not_exist_is_reported_and_left_out(what):
     if what in ("page", "negative page"):
         with pytest.raises(RuntimeError, match="does not exist"):
             cache.read(table, T)
-        with pytest.raises(RuntimeError, match="does not exist"):
-            cache.attend(tensor(seeded(3, B, H, 1, d)), table, [T])
+        for heads in (1, 40):
+            with pytest.raises(RuntimeError, match="does not exist"):
+                cache.attend(tensor(seeded(3, B, H * heads, 2, d).astype(np.float16)), table, [T])
     _lib.check(_lib.load().tx_sdpa_finish(None))
 
 
@@ -146,13 +147,17 @@ def words_of(shape, seed, B, T):
     return words, words
 
 
-def check_attention(got, q, kv, kv_lens, q_lens, words, window, sinks, fp32, out16):
+def check_attention(got, q, kv, kv_lens, q_lens, words, window, sinks, fp32, out16, fp16_cache=False):
     """Every element within what the roundings of the products can make of it.
 
     fp16 queries: a weight is rounded to fp16 (2^-11 of it); the score's sum of d products in fp32 may lose 2^-23 of the
     sum of their sizes per addition (matrix units cut off), `e` in all; both the weight and the sum of the weights carry e.
     fp32: a weight is two fp16 numbers (2^-22), so is a query (2^-22 per product).  2^-19: the exponential (2^-22), the
-    scales' products and the partial sums.  fp16 results are rounded once more."""
+    scales' products and the partial sums.  fp16 results are rounded once more.
+    fp16_cache: many rows a head; keys and values times their scales are rounded to fp16 (2^-11 of a product, of a value; an
+    element below 2^-14 of 224 in the tile's largest row, to 2^-25 of that: 2^-30 of the largest value), and the exponential may be the
+    polynomial one (2^-12.5 in weight and sum).  Weights more than 2^24 (and 2^8 for a maximum not yet raised) below the
+    row's largest are lost: with up to 2^10 keys in a tile's row, 2^-7 of that at most here, 2^-17 of the largest value."""
     B, Hq, T, d = q.shape
     G = Hq // kv[0].shape[1]
     for b in range(B):
@@ -164,10 +169,24 @@ def check_attention(got, q, kv, kv_lens, q_lens, words, window, sinks, fp32, out
             assert np.array_equal(np.isnan(have), np.isnan(want)), (b, h)
             e = size * (d * 2.0 ** -23 * (2 if fp32 else 1) + 2.0 ** -22)
             bound = weight * ((2.0 ** -21 if fp32 else 2.0 ** -11) + 2 * e[:, None] + 2.0 ** -19) + 1e-30
+            if fp16_cache:
+                top = np.abs(kv[1][b, h // G, : kv_lens[b]]).max(initial=0.0)
+                bound = bound + weight * (2.0 ** -11 + 2.0 ** -11.5 + 2 * 2.0 ** -11 * size[:, None]) + 2.0 ** -17 * top
             if out16:
                 bound = bound + np.abs(want) * 2.0 ** -11 + 2.0 ** -25
             assert (np.abs(have - want) <= bound)[~np.isnan(want)].all(), (b, h, np.nanmax(np.abs(have - want) / bound))
 
+
+MANY = [
+    # as CASES below; more than 64 rows a head: the tcgen05 kernel
+    (1, 8, 1, 64, 64, 16, None, None, 0, "tree"),               # two query tiles, no context
+    (2, 5, 1, 13, 1, 16, [1, 0], None, 0, "tree"),              # one key; one sequence without nodes
+    (2, 3, 1, 23, 300, 32, [23, 7], None, 0, "chain"),          # one query tile, three tiles of keys
+    (1, 6, 2, 64, 513, 64, None, 130, 70, "tree"),              # sinks and window apart, nodes over two tiles
+    (2, 16, 2, 33, 2000, 128, [33, 12], 700, 5, "tree"),        # two parts of 256 rows
+    (1, 4, 1, 64, 4100, 256, None, 3000, 200, "chain"),
+    (1, 4, 1, 50, 1030, 16, None, 64, 0, "tree"),
+]
 
 CASES = [
     # B, Hq, Hkv, T, S (keys of the longest sequence), page, q_lens, window, sinks, shape
@@ -198,9 +217,29 @@ def test_attention(case, d, dtype, fmt):
         out = cache.attend(tensor(q), table, kv_lens, q_lens=q_lens, tree=tree, window=window, sinks=sinks, out_dtype=out_dtype)
         assert out.dtype == out_dtype
         got = out.numpy()
-        check_attention(got, q, kv, kv_lens, nodes, words, window, sinks, dtype == np.float32, out_dtype == "float16")
+        check_attention(got, q, kv, kv_lens, nodes, words, window, sinks, dtype == np.float32, out_dtype == "float16",
+                        fp16_cache=dtype == np.float16 and d <= 128 and Hq // Hkv * T > 64)
         for b in range(B):
             assert (got[b, :, nodes[b]:] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_attention_of_many_rows(case, d, fmt):
+    B, Hq, Hkv, T, S, page, q_lens, window, sinks, shape = MANY[case]
+    cache, table, kv = filled(200 + case, B, Hkv, S, d, page, fmt)
+    q = seeded(case, B, Hq, T, d).astype(np.float16)
+    nodes = [min(n, S) for n in (q_lens or [T] * B)]
+    kv_lens = [S - 37 * b if S - 37 * b >= max(nodes[b], 1) else S for b in range(B)]
+    tree, words = words_of(shape, case, B, T)
+    for out_dtype in ("float32", "float16"):
+        got = cache.attend(tensor(q), table, kv_lens, q_lens=q_lens, tree=tree, window=window, sinks=sinks, out_dtype=out_dtype).numpy()
+        check_attention(got, q, kv, kv_lens, nodes, words, window, sinks, False, out_dtype == "float16", fp16_cache=True)
+        for b in range(B):
+            assert (got[b, :, nodes[b]:] == 0).all()
+    again = cache.attend(tensor(q), table, kv_lens, q_lens=q_lens, tree=tree, window=window, sinks=sinks, out_dtype="float16").numpy()
+    assert np.array_equal(got, again, equal_nan=True)
 
 
 def test_fp32_queries_keep_fp32_accuracy():
@@ -221,6 +260,10 @@ def test_a_node_that_sees_nothing_and_words_of_all_bits():
     got = cache.attend(tensor(q), table, [64], tree=words).numpy()
     assert np.isnan(got[0, 0, 0]).all() and np.isnan(got[0, 0, 2:63]).all()
     check_attention(got, q, kv, [64], [64], words, None, 0, False, False)
+    q = seeded(4, 1, 2, 64, 64).astype(np.float16)                # 128 rows
+    got = cache.attend(tensor(q), table, [64], tree=words).numpy()
+    assert np.isnan(got[0, :, 0]).all() and np.isnan(got[0, :, 2:63]).all()
+    check_attention(got, q, kv, [64], [64], words, None, 0, False, False, fp16_cache=True)
 
 
 def test_values_of_any_magnitude():
@@ -236,6 +279,10 @@ def test_values_of_any_magnitude():
             kv = [kv_oracle.values(*kv_oracle.quantise(x, fmt), fmt) for x in (k, mixed)]
             q = seeded(3, B, 4, 1, d).astype(np.float16)
             check_attention(cache.attend(tensor(q), table, [S]).numpy(), q, kv, [S], [1], [[1]], None, 0, False, False)
+            q = seeded(3, B, 16, 6, d).astype(np.float16)
+            got = cache.attend(tensor(q), table, [S]).numpy()
+            words = [[(2 << t) - 1 for t in range(6)]]
+            check_attention(got, q, kv, [S], [6], words, None, 0, False, False, fp16_cache=True)
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
@@ -251,11 +298,12 @@ def test_what_is_not_finite_stays_where_it_is_seen(fmt):
     cache = QuantizedKVCache(10, H, d, page, fmt)
     cache.write(tensor(k), tensor(v), table)
     tree = np.array([[0b001, 0b011, 0b101]], np.uint64)
-    q = seeded(3, B, 2, T, d).astype(np.float16)
-    got = cache.attend(tensor(q), table, [S], tree=tree, window=window).numpy()
-    assert np.isfinite(got[0, :, 0]).all() and np.isnan(got[0, :, 1]).all() and np.isnan(got[0, :, 2]).all()
-    kv = [np.nan_to_num(kv_oracle.values(*kv_oracle.quantise(x, fmt), fmt)) for x in (k, v)]
-    check_attention(got[:, :, :1], q[:, :, :1], kv, [148], [1], [[1]], window, 0, False, False)
+    for heads in (2, 40):                        # 6 rows, and 120
+        q = seeded(3, B, heads, T, d).astype(np.float16)
+        got = cache.attend(tensor(q), table, [S], tree=tree, window=window).numpy()
+        assert np.isfinite(got[0, :, 0]).all() and np.isnan(got[0, :, 1]).all() and np.isnan(got[0, :, 2]).all()
+        kv = [np.nan_to_num(kv_oracle.values(*kv_oracle.quantise(x, fmt), fmt)) for x in (k, v)]
+        check_attention(got[:, :, :1], q[:, :, :1], kv, [148], [1], [[1]], window, 0, False, False, fp16_cache=heads > 2)
 
 
 def test_queries_that_are_not_finite():
