@@ -86,12 +86,12 @@ int move_rows(const char *who, const tx_kv_cache &c, const void *k, const void *
     if (int rc = txb::api::status_word(&p.status)) return rc;
     p.k = const_cast<void *>(k); p.v = const_cast<void *>(v);
     p.start = start; p.counts = counts; p.pick = pick;
-    p.rows = batch * c.kv_heads * tokens;
     p.tokens = (int)tokens; p.src_tokens = (int)src_tokens;
     return for_types(dtype, c.format, c.d, [&](auto t, auto fmt, auto d) -> int {
         using T = decltype(t);
-        constexpr int per_cta = txb::KV_MOVE_THREADS / (d() / 8) * txb::KV_MOVE_STEPS;
-        const int64_t ctas = (p.rows + per_cta - 1) / per_cta;
+        constexpr int per_cta = txb::KvMoveItem<d()>::PER_CTA;
+        p.ctas = (int)((tokens + per_cta - 1) / per_cta);
+        const int64_t ctas = batch * c.kv_heads * p.ctas;
         if (ctas > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "%s: dimension too large", who);
         const cudaStream_t st = static_cast<cudaStream_t>(stream);
         if constexpr (WRITE) txb::kv_write_kernel<T, fmt(), d()><<<(unsigned)ctas, txb::KV_MOVE_THREADS, 0, st>>>(p);
