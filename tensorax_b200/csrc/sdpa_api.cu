@@ -735,7 +735,10 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
             tk = std::min(tk, up((int64_t)win->window + DkvCfg::BMK, DkvCfg::BQ) * ratio);
             if (win->sinks > 0 && all > 2.0 * tk) {
                 sink_tiles = std::min<int64_t>((win->sinks + DkvCfg::BMK - 1) / DkvCfg::BMK, (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK);
-                while (split_sinks < 8 && all / split_sinks > tk) split_sinks *= 2;
+                // (to no longer than the others, and further while there are SMs without a CTA: B2 Hq12 Hkv4 S921 d64 44 us a
+                // launch in four, SINKS8 in eight)
+                const int64_t ctas = sink_tiles * d->batch * d->kv_heads * DkvCfg::ZS;
+                while (split_sinks < 8 && (all / split_sinks > tk || ctas * split_sinks * 2 <= (int64_t)DkvCfg::CTAS_PER_SM * sms)) split_sinks *= 2;
             }
         }
         const bool uneven = d->causal && !win;           // half of the tiles on average

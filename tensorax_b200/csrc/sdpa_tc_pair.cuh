@@ -145,13 +145,16 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool live1 = q0 + BM < p.Sq;
     const int kv_end0 = p.causal ? min(kv_limit, q0 + BM) : kv_limit;
     const int kv_end1 = live1 ? (p.causal ? min(kv_limit, q0 + 2 * BM) : kv_limit) : 0;
-    // With a window both tiles walk one list, that of all their rows: the second one's first entry may be masked as a
-    // whole (one tile of window / BN + 2), which costs less than two rings.
+    // With a window both tiles walk one list, that of all their rows; the first entry behind the sinks may hold keys of the
+    // first tile's windows only, and the second tile then leaves it out (`gone`, else -1): it walks entry j as its own number j1.
     const int off = Cfg::WINDOW ? p.win.offset(kv_limit, p.Sq) : 0;
     const WindowWalk<BN> walk(p.win, kv_limit, off + q0, live1 ? 2 * BM : BM);
     const int n0 = Cfg::WINDOW ? walk.count_below(off + q0 + BM) : (kv_end0 + BN - 1) / BN;
     const int n1 = Cfg::WINDOW ? (live1 ? walk.count() : 0) : (kv_end1 + BN - 1) / BN;
     auto tile_of = [&](int j) { return Cfg::WINDOW ? walk.tile(j) : j; };
+    const bool second_sees = !Cfg::WINDOW || walk.w_tile >= walk.end ||
+                             (walk.w_tile + 1) * BN > max(off + q0 + BM - p.win.window + 1, 0) || walk.w_tile * BN < p.win.sinks;
+    const int gone = Cfg::WINDOW && !second_sees && n0 > walk.n_sink && n1 > walk.n_sink + 1 ? walk.n_sink : -1;
     const int n_max = max(n0, n1);
 
     // Warp 0 sets the barriers up and sends the first loads (both Q tiles, K and V of key tile 0) on their way
@@ -278,6 +281,8 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             tick_start();
             const long long t_begin = Cfg::PROF ? clock64() : 0;
             long long t_q = 0, t_k0 = 0;
+            auto own = [&](int t, int j) { return Cfg::WINDOW && t == 1 && gone >= 0 && j > gone ? j - 1 : j; };
+            auto walks = [&](int t, int j) { return !(Cfg::WINDOW && t == 1 && j == gone); };
             // S_t = Q_t K_j^T; the K stage is released by whichever tile reads it last
             auto issue_qk = [&](int t, int j) -> bool {
                 const int s = j % NS;
@@ -290,7 +295,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const uint32_t ks_lo = k_lo + (uint32_t)s * (Cfg::K_BYTES >> 4);
                 const uint32_t qt_lo = q_lo + (uint32_t)t * (Cfg::Q_TILE_BYTES >> 4);
                 const uint32_t t_s = tmem + (t ? Cfg::COL_S1 : Cfg::COL_S0);
-                const bool last_reader = t == 1 ? true : (j >= n1);
+                const bool last_reader = t == 1 ? true : (j >= n1 || (Cfg::WINDOW && j == gone));
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
@@ -313,18 +318,19 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 tick(0);
                 if (!ptx::mbar_wait(v_full + 8 * s, ph, abort_flag, Cfg::WAIT_NS)) return false;
                 tick(4);
-                if (!ptx::mbar_wait(p_full + 8 * t, (uint32_t)j & 1u, abort_flag, Cfg::WAIT_NS)) return false;
+                const int j1 = own(t, j);
+                if (!ptx::mbar_wait(p_full + 8 * t, (uint32_t)j1 & 1u, abort_flag, Cfg::WAIT_NS)) return false;
                 tick(3);
                 ptx::tc_fence_after_sync();
                 const uint32_t vs_lo = v_lo + (uint32_t)s * (Cfg::V_BYTES >> 4);
                 const uint32_t t_o = tmem + (t ? Cfg::COL_O1 : Cfg::COL_O0);
                 const uint32_t t_p = tmem + (t ? Cfg::COL_P1 : Cfg::COL_P0);
-                const bool last_reader = t == 1 ? true : (j >= n1);
+                const bool last_reader = t == 1 ? true : (j >= n1 || (Cfg::WINDOW && j == gone));
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk) {
                         const uint64_t bdesc = ptx::make_desc(vs_lo + kk * ((16 * 128) >> 4), desc_hi);
-                        ptx::mma_ts(t_o, t_p + kk * 8, bdesc, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                        ptx::mma_ts(t_o, t_p + kk * 8, bdesc, idesc_pv, (j1 > 0 || kk > 0) ? 1u : 0u);
                     }
                     if (last_reader) ptx::mma_commit(v_empty + 8 * s);
                     ptx::mma_commit(pv_done + 8 * t);
@@ -340,24 +346,25 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             }
             if (ok && n1 > 0) {
                 ok = ptx::mbar_wait(q_full + 8, 0, abort_flag, Cfg::WAIT_NS);
-                if (ok) ok = issue_qk(1, 0);
+                if (ok && walks(1, 0)) ok = issue_qk(1, 0);
             }
             for (int j = 0; j < n_max && ok; ++j) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int nt = t ? n1 : n0;
                     if constexpr (!Cfg::P_ALIAS) {
-                        if (j + 1 < nt && ok) {
+                        if (j + 1 < nt && ok && walks(t, j + 1)) {
                             tick(0);
-                            ok = ptx::mbar_wait(s_free + 8 * t, (uint32_t)j & 1u, abort_flag, Cfg::WAIT_NS);
+                            const int j1 = own(t, j + 1) - 1;       // whose S is handed back first (none before the tile's first)
+                            if (!Cfg::WINDOW || j1 >= 0) ok = ptx::mbar_wait(s_free + 8 * t, (uint32_t)j1 & 1u, abort_flag, Cfg::WAIT_NS);
                             tick(1);
                             if (ok) { ptx::tc_fence_after_sync(); ok = issue_qk(t, j + 1); }
                         }
-                        if (j < nt && ok) ok = issue_pv(t, j);
+                        if (j < nt && ok && walks(t, j)) ok = issue_pv(t, j);
                     } else {
                         // P_t lives in S_t's columns: the next QK^T of this tile follows its PV in program order
-                        if (j < nt && ok) ok = issue_pv(t, j);
-                        if (j + 1 < nt && ok) ok = issue_qk(t, j + 1);
+                        if (j < nt && ok && walks(t, j)) ok = issue_pv(t, j);
+                        if (j + 1 < nt && ok && walks(t, j + 1)) ok = issue_qk(t, j + 1);
                     }
                 }
             }
@@ -385,7 +392,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int r = quarter * 32 + lane;               // row inside the tile
         const int q0t = q0 + t * BM;
         const int row = q0t + r;
-        const int nt = t ? n1 : n0;
+        const int skipped = Cfg::WINDOW && t == 1 ? gone : -1, nt = (t ? n1 : n0) - (skipped >= 0 ? 1 : 0);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t t_s = tmem + lane_base + (t ? Cfg::COL_S1 : Cfg::COL_S0);
         const uint32_t t_o = tmem + lane_base + (t ? Cfg::COL_O1 : Cfg::COL_O0);
@@ -405,7 +412,8 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         tick_start();
         const long long t_begin = Cfg::PROF ? clock64() : 0;
         for (int j = 0; j < nt && ok; ++j) {
-            const int kv0 = tile_of(j) * BN;
+            const int entry = Cfg::WINDOW && skipped >= 0 && j >= skipped ? j + 1 : j;
+            const int kv0 = tile_of(entry) * BN;
             tick(0);
             ok = ptx::mbar_wait(my_s_full, (uint32_t)j & 1u, abort_flag, Cfg::WAIT_NS);
             tick(PSEC_SM_WAIT_S);
@@ -487,11 +495,11 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 }
             }
             tick(PSEC_SM_WAIT_PV);
-            if (Cfg::WINDOW && kv0 + BN > kv_limit && (t == 0 || j >= n0)) {
+            if (Cfg::WINDOW && kv0 + BN > kv_limit && (t == 0 || entry >= n0)) {
                 // what lies behind the sequence's last key; query tile 0's PV comes before tile 1's, so its warps do it for both
-                ok = ptx::mbar_wait(v_full + 8 * (j % NS), (uint32_t)(j / NS) & 1u, abort_flag, Cfg::WAIT_NS);
+                ok = ptx::mbar_wait(v_full + 8 * (entry % NS), (uint32_t)(entry / NS) & 1u, abort_flag, Cfg::WAIT_NS);
                 if (!ok) break;
-                zero_stage_rows<BN, 128>(smem + Cfg::OFF_V + (j % NS) * Cfg::V_BYTES, Cfg::KP, kv_limit - kv0, r);
+                zero_stage_rows<BN, 128>(smem + Cfg::OFF_V + (entry % NS) * Cfg::V_BYTES, Cfg::KP, kv_limit - kv0, r);
                 ptx::fence_proxy_async_smem();
             }
             ptx::tmem_st_cols<BN / 2>(t_p, pk);

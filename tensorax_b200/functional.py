@@ -155,12 +155,13 @@ def scaled_dot_product_attention_ex(query: Tensor, key: Tensor, value: Tensor,
 def scaled_dot_product_attention_window(query: Tensor, key: Tensor, value: Tensor, window: int, sinks: int = 0,
                                         kv_lens: Optional[Sequence[int]] = None, align: str = "start",
                                         out_dtype: str = "float32", grad_dtype: str = "float32",
-                                        sync: bool = True) -> Tensor:
+                                        sync: Optional[bool] = None) -> Tensor:
     """No reference counterpart.  Causal attention with a sliding window: row i at position p sees key j iff j <= p,
     j < kv_lens[b], and j > p - window or j < sinks (first keys that stay visible).  ``align="start"``: p = i;
     ``align="end"``: the rows are the last ones of their sequence, p = kv_lens[b] - Sq + i (a decoding step, or a chunk of
     a long prompt).  K/V may have fewer heads than Q; float16 and float32.  A row that sees no key is NaN.  Differentiable
-    for float16 with d in {64, 128, 256}; ``grad_dtype="float16"`` leaves the gradients in float16."""
+    for float16 with d in {64, 128, 256}; ``grad_dtype="float16"`` leaves the gradients in float16.  ``sync``: wait for
+    the result; by default unless it is recorded for ``backward``, which waits (so does any download, or ``synchronize()``)."""
     _check(query, key, value, None, _MSG4D)
     if grad_dtype not in ("float32", "float16"):
         raise ValueError("grad_dtype must be 'float32' or 'float16'")
@@ -168,11 +169,13 @@ def scaled_dot_product_attention_window(query: Tensor, key: Tensor, value: Tenso
         raise RuntimeError("C++ backend not available.")
     q, k, v = query._c_tensor, key._c_tensor, value._c_tensor
     needs_grad = query.requires_grad or key.requires_grad or value.requires_grad
+    recorded = needs_grad and _C.sdpa_backward_supported(q, k, v, None)
+    sync = not recorded if sync is None else sync
     if not needs_grad:
         return _result(_C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens,
                                                               out_dtype=out_dtype, sync=sync))
     grad_fn = ("scaled_dot_product_attention", query, key, value, None)
-    if not _C.sdpa_backward_supported(q, k, v, None):
+    if not recorded:
         return _result(_C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens,
                                                               out_dtype=out_dtype, sync=sync), True, grad_fn)
     c, lse = _C.scaled_dot_product_attention_window(q, k, v, window, sinks, align, kv_lens=kv_lens, out_dtype=out_dtype,
