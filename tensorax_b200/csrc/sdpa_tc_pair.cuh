@@ -28,6 +28,8 @@
 #include "ptx.cuh"
 #include "sdpa_tc.cuh"
 
+#include <type_traits>
+
 namespace txb {
 
 // Section profile of this kernel: cycles per step, summed over key tiles, for one softmax lane of either
@@ -155,6 +157,9 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     const bool second_sees = !Cfg::WINDOW || walk.w_tile >= walk.end ||
                              (walk.w_tile + 1) * BN > max(off + q0 + BM - p.win.window + 1, 0) || walk.w_tile * BN < p.win.sinks;
     const int gone = Cfg::WINDOW && !second_sees && n0 > walk.n_sink && n1 > walk.n_sink + 1 ? walk.n_sink : -1;
+    // A tile that is walked for up to 32 sinks alone is as narrow as that: entry 0 then takes a quarter of the products and
+    // exponentials (its loads stay whole: they run ahead).
+    const bool narrow = Cfg::WINDOW && walk.n_sink == 1 && p.win.sinks <= 32;
     const int n_max = max(n0, n1);
 
     // Warp 0 sets the barriers up and sends the first loads (both Q tiles, K and V of key tile 0) on their way
@@ -271,7 +276,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         // P_ALIAS relies on (the QK^T that overwrites S/P follows the PV that read P).
         if (run) {
             const bool leader = ptx::elect_one();
-            constexpr uint32_t idesc_qk = ptx::idesc_f16(BM, BN, false);
+            constexpr uint32_t idesc_qk_all = ptx::idesc_f16(BM, BN, false), idesc_qk_32 = ptx::idesc_f16(BM, 32, false);
             constexpr uint32_t idesc_pv = ptx::idesc_f16(BM, D, true);
             constexpr uint32_t desc_hi = ptx::smem_desc_sw128_hi(1024);
             const uint32_t q_lo = ptx::smem_desc_sw128_lo(q_s, 16);
@@ -296,6 +301,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const uint32_t qt_lo = q_lo + (uint32_t)t * (Cfg::Q_TILE_BYTES >> 4);
                 const uint32_t t_s = tmem + (t ? Cfg::COL_S1 : Cfg::COL_S0);
                 const bool last_reader = t == 1 ? true : (j >= n1 || (Cfg::WINDOW && j == gone));
+                const uint32_t idesc_qk = narrow && j == 0 ? idesc_qk_32 : idesc_qk_all;
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
@@ -329,6 +335,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 if (leader) {
 #pragma unroll
                     for (int kk = 0; kk < BN / 16; ++kk) {
+                        if (Cfg::WINDOW && kk == 2 && narrow && j == 0) break;
                         const uint64_t bdesc = ptx::make_desc(vs_lo + kk * ((16 * 128) >> 4), desc_hi);
                         ptx::mma_ts(t_o, t_p + kk * 8, bdesc, idesc_pv, (j1 > 0 || kk > 0) ? 1u : 0u);
                     }
@@ -411,22 +418,24 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const bool prof_lane = prof_on && quarter == 0 && lane == 0;
         tick_start();
         const long long t_begin = Cfg::PROF ? clock64() : 0;
-        for (int j = 0; j < nt && ok; ++j) {
+        // one tile of keys, the first CN of its columns
+        auto walk_tile = [&](auto cn, int j) -> bool {
+            constexpr int CN = decltype(cn)::value;
             const int entry = Cfg::WINDOW && skipped >= 0 && j >= skipped ? j + 1 : j;
             const int kv0 = tile_of(entry) * BN;
             tick(0);
             ok = ptx::mbar_wait(my_s_full, (uint32_t)j & 1u, abort_flag, Cfg::WAIT_NS);
             tick(PSEC_SM_WAIT_S);
             if constexpr (Cfg::PROF) { if (j == 0 && prof_lane) p.prof[(t ? 32 : 0) + PSEC_SM_FIRST_S] = clock64() - t_entry; }
-            if (!ok) break;
+            if (!ok) return false;
             ptx::tc_fence_after_sync();
             // The whole score row goes to registers with one wait.  The array is defined here, inside the
             // loop, by this one load: a row kept alive across the loop edge (loaded at the bottom for the
             // next iteration) cost a register shuffle per tile and 20 % of the kernel's speed.
-            uint32_t sv[BN];
-            ptx::tmem_ld_cols<BN>(t_s, sv);
+            uint32_t sv[CN];
+            ptx::tmem_ld_cols<CN>(t_s, sv);
             ptx::tmem_wait_ld();
-            ptx::reg_fence_cols<BN>(sv);
+            ptx::reg_fence_cols<CN>(sv);
             if constexpr (!Cfg::P_ALIAS) arrive_warp(my_s_free);   // S belongs to the MMA warp again
             tick(PSEC_SM_LOAD_S);
             const bool need_mask = Cfg::WINDOW ? window_edge(p.win, kv_limit, off + q0t, BM, kv0, BN)
@@ -434,17 +443,17 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (Cfg::WINDOW && need_mask) {
                 const WindowColumns seen(p.win, kv_limit, off + row, kv0);
 #pragma unroll
-                for (int i = 0; i < BN; ++i) sv[i] = keep_if_seen(sv[i], i, seen);
+                for (int i = 0; i < CN; ++i) sv[i] = keep_if_seen(sv[i], i, seen);
             } else if (need_mask) {
                 // visible keys of this row are a prefix of the tile: columns [0, lim)
                 const int lim = min(kv_limit - kv0, p.causal ? row - kv0 + 1 : BN);
 #pragma unroll
-                for (int i = 0; i < BN; ++i) sv[i] = ptx::keep_if_below(sv[i], i, lim);
+                for (int i = 0; i < CN; ++i) sv[i] = ptx::keep_if_below(sv[i], i, lim);
             }
             tick(PSEC_SM_MASK);
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < BN; i += 8) {
+            for (int i = 0; i < CN; i += 8) {
                 mx0 = ptx::max3(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
                 mx1 = ptx::max3(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
                 mx2 = ptx::max3(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
@@ -458,9 +467,9 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             // p = 2^(s*scale - m): a masked score is -inf and gives exactly 0
             const float2 scale2 = make_float2(scale, scale), negm2 = make_float2(-m_next, -m_next);
             float2 sum_a = make_float2(0.f, 0.f), sum_b = make_float2(0.f, 0.f);
-            uint32_t pk[BN / 2];
+            uint32_t pk[CN / 2];
 #pragma unroll
-            for (int i = 0; i < BN; i += 4) {
+            for (int i = 0; i < CN; i += 4) {
                 const float2 xa = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), scale2, negm2);
                 const float2 xb = __ffma2_rn(make_float2(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])), scale2, negm2);
                 const int e0 = i & 15;
@@ -478,7 +487,7 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 // PV of the previous tile must be finished before P is overwritten or O rescaled (with P in
                 // S's columns the scores themselves came after it, so this wait returns at once)
                 ok = ptx::mbar_wait(my_pv_done, (uint32_t)(j - 1) & 1u, abort_flag, Cfg::WAIT_NS);
-                if (!ok) break;
+                if (!ok) return false;
                 ptx::tc_fence_after_sync();
                 if (__any_sync(0xffffffffu, alpha != 1.0f)) {
                     // rare after the first tiles; 16 columns at a time
@@ -498,14 +507,19 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             if (Cfg::WINDOW && kv0 + BN > kv_limit && (t == 0 || entry >= n0)) {
                 // what lies behind the sequence's last key; query tile 0's PV comes before tile 1's, so its warps do it for both
                 ok = ptx::mbar_wait(v_full + 8 * (entry % NS), (uint32_t)(entry / NS) & 1u, abort_flag, Cfg::WAIT_NS);
-                if (!ok) break;
+                if (!ok) return false;
                 zero_stage_rows<BN, 128>(smem + Cfg::OFF_V + (entry % NS) * Cfg::V_BYTES, Cfg::KP, kv_limit - kv0, r);
                 ptx::fence_proxy_async_smem();
             }
-            ptx::tmem_st_cols<BN / 2>(t_p, pk);
+            ptx::tmem_st_cols<CN / 2>(t_p, pk);
             ptx::tmem_wait_st();
             arrive_warp(my_p_full);
             tick(PSEC_SM_STORE_P);
+            return true;
+        };
+        for (int j = 0; j < nt && ok; ++j) {
+            if (Cfg::WINDOW && narrow && j == 0) ok = walk_tile(std::integral_constant<int, Cfg::WINDOW ? 32 : BN>{}, j);
+            else ok = walk_tile(std::integral_constant<int, BN>{}, j);
         }
         const long long t_loop_end = Cfg::PROF ? clock64() : 0;
         if (run && nt > 0 && ok) {
