@@ -869,6 +869,8 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             // that none of them is left behind at it.
             const int qr0 = (i_start + i_n) * BQ;
             float *st_lse = stat + (t & 1) * 2 * BQ, *st_delta = st_lse + BQ;
+            // (a row that sees no key, window: its sum is nothing and its maximum the stand-in, its delta 0/0)
+            if (Cfg::WINDOW && (st < BQ ? next_stat < -1.0e29f : next_stat != next_stat)) next_stat = st < BQ ? INFINITY : 0.f;
             if (st < 2 * BQ) st_lse[st] = stat_mul * next_stat;
             if constexpr (Cfg::WGS == 1) asm volatile("bar.sync 1, 128;" ::: "memory");
             else asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -891,8 +893,9 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             arrive_warp(s_free);
             const int qc0 = qr0 + c0;               // first query of this warpgroup's columns
             // columns of the tile whose queries see this key: from its own position on, as far as its window goes
-            const int seen_lo = key - off - qc0, seen_hi = key < p.win.sinks ? CW : min(CW, seen_lo + p.win.window);
-            const bool need_mask = Cfg::WINDOW ? (key0 + BMK - 1 > off + qc0 || key0 + BMK > kv_limit ||
+            const bool last_keys = key0 + BMK > kv_limit;
+            const int seen_lo = key - off - qc0, seen_hi = !key_ok ? -1 : key < p.win.sinks ? CW : min(CW, seen_lo + p.win.window);
+            const bool need_mask = Cfg::WINDOW ? (key0 + BMK - 1 > off + qc0 || last_keys ||
                                                   (off + qc0 + CW - 1 >= key0 + p.win.window && key0 + BMK > p.win.sinks))
                                                : p.causal && (key0 + BMK - 1 > qc0);
             const int key_lo = key - qc0 - 1;
@@ -905,6 +908,10 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const float2 dl = *reinterpret_cast<const float2 *>(st_delta + c0 + i);
                 const float2 x = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])), c2, l2);
                 float2 pr = make_float2(ptx::ex2_approx(x.x), ptx::ex2_approx(x.y));
+                if (Cfg::WINDOW && need_mask) {
+                    pr.x = zero_unless_within(pr.x, i, seen_lo, seen_hi);
+                    pr.y = zero_unless_within(pr.y, i + 1, seen_lo, seen_hi);
+                }
                 if (!Cfg::WINDOW && !key_ok) pr = make_float2(0.f, 0.f);
                 if (!Cfg::WINDOW && need_mask) { // query qc0 + i sees this key when key <= qc0 + i
                     pr.x = ptx::zero_unless_lt(pr.x, key_lo, i);
@@ -913,13 +920,7 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 const float2 tt = __ffma2_rn(make_float2(__uint_as_float(dpv[i]), __uint_as_float(dpv[i + 1])), s2,
                                              dl);
                 float2 ds = __fmul2_rn(pr, tt);
-                if (Cfg::WINDOW && need_mask) {  // both: a query that sees nothing has no statistics, a key behind the last no value
-                    const int hi = key_ok ? seen_hi : -1;
-                    pr.x = zero_unless_within(pr.x, i, seen_lo, hi);
-                    pr.y = zero_unless_within(pr.y, i + 1, seen_lo, hi);
-                    ds.x = zero_unless_within(ds.x, i, seen_lo, hi);
-                    ds.y = zero_unless_within(ds.y, i + 1, seen_lo, hi);
-                }
+                if (Cfg::WINDOW && last_keys && !key_ok) ds = make_float2(0.f, 0.f);     // whatever V holds there
                 pp[i / 2] = ptx::pack_half2(pr.x, pr.y);
                 pd[i / 2] = ptx::pack_half2(ds.x, ds.y);
             }
