@@ -505,7 +505,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
     if (warp >= 8) {
         constexpr int QUADS = D / 4, S = Cfg::MAX_SPLITS, RPW = 32 / QUADS > 0 ? 32 / QUADS : 1;    // rows a warp takes side by side
         float *worth = reinterpret_cast<float *>(smem + Cfg::OFF_CODES);         // [row of the share][CTA]
-        const int mine = MR / splits, r_first = split * mine;
+        const int row_share = (MR + splits - 1) / splits, r_first = split * row_share, mine = min(row_share, MR - r_first);
         if (tid - 256 < mine) {
             const int r = r_first + tid - 256;
             float2 s[S];
