@@ -39,6 +39,7 @@
 #include "sdpa_tc_x3.cuh"
 #include "sdpa_simt.cuh"
 #include "sdpa_bwd.cuh"
+#include "sdpa_bwd_sinks.cuh"
 #include "sdpa_decode.cuh"
 #include "api_internal.h"
 
@@ -703,6 +704,36 @@ double bwd_together(const BwdWork &q, int zq, const BwdWork &k, int zk, int sms)
     return std::max({work, behind + chain(k, zk), chain(q, zq)});
 }
 
+// Sinks of a windowed call whose gradients the kernel of sixteen keys takes, d = 64 and 128.  The backward call with four, 16
+// and 32 of them, in us, against the launch of whole key tiles: B4 H16 S2048 d128 window 512 252, 255, 274 and 259, 267, 268;
+// B8 H16 S2048 d64 window 256 250, 250, 265 and 288, 288, 289.  B2 Hq8 Hkv2 S4096 d256 window 512 442, 439, 462 and 444, 439, 439.
+constexpr int kSinkKeys = 16;
+
+template <class Cfg>
+int launch_sink_grads(const tx_sdpa_bwd_desc *d, cudaStream_t st, const __half *dout_h, const float *delta, int *prepared,
+                      const txb::WindowRule &win)
+{
+    txb::SinkGradParams p;
+    p.q = static_cast<const __half *>(d->q); p.k = static_cast<const __half *>(d->k); p.v = static_cast<const __half *>(d->v);
+    p.dout = dout_h; p.lse = d->lse; p.delta = delta;
+    p.kv_lens = lens_of(d->kv_lens, d->flags, d->batch);
+    p.dk = d->dk; p.dv = d->dv; p.prepared = prepared;
+    p.win = win;
+    p.Hkv = (int)d->kv_heads; p.group = (int)(d->q_heads / d->kv_heads); p.Sq = (int)d->seq_q; p.Sk = (int)d->seq_k;
+    p.grads_f16 = (d->flags & TX_BWD_GRADS_F16) ? 1 : 0;
+    p.scale = 1.0f / std::sqrt((float)Cfg::D);
+    p.scale_log2 = p.scale * 1.4426950408889634f;
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    // the rows of an item over the CTAs of a cluster: as many as one wave holds and as have a step for each of their warps
+    const int64_t items = d->batch * d->kv_heads, steps = ((int64_t)p.group * p.Sq + 15) / 16;
+    int splits = 1;
+    while (splits < 8 && items * splits * 2 <= (int64_t)Cfg::CTAS_PER_SM * sms && (int64_t)splits * Cfg::WARPS < steps) splits *= 2;
+    if (items * splits > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "SDPA backward: more than 2^31 work items");
+    if (int rc = allow_smem<txb::sdpa_bwd_sinks_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
+    return launch_behind(txb::sdpa_bwd_sinks_kernel<Cfg>, dim3((unsigned)(items * splits)), Cfg::THREADS, Cfg::SMEM, st, splits, p);
+}
+
 template <int D, class DqCfg, class DkvCfg>
 int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __half *dout_h, const float *delta, int *prepared,
                const txb::WindowRule *win = nullptr)
@@ -722,7 +753,9 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
     if (int rc = sm_count(&sms)) return rc;
     if (win) { p.win = *win; p.grads_f16 = (d->flags & TX_BWD_GRADS_F16) ? 1 : 0; }
     // With a window a key tile is seen by the rows of its window, the tiles of the sinks by all rows.  Where that makes them
-    // much longer than the others they get a launch of their own, cut over clusters, in front of the others.
+    // much longer than the others, up to kSinkKeys sinks go to a kernel of their own, more of them to a launch of the same kernel
+    // in front of the others, cut over clusters.
+    bool sinks_apart = false;
     int64_t sink_tiles = 0;
     int split_sinks = 1;
     {
@@ -733,10 +766,10 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
             const double all = tk;
             tq = std::min(tq, up((int64_t)win->window + DqCfg::BM, DqCfg::BN) + up(std::min<int64_t>(win->sinks, d->seq_k), DqCfg::BN));
             tk = std::min(tk, up((int64_t)win->window + DkvCfg::BMK, DkvCfg::BQ) * ratio);
-            if (win->sinks > 0 && all > 2.0 * tk) {
+            if (win->sinks > 0 && all > 2.0 * tk) sinks_apart = D <= 128 && win->sinks <= kSinkKeys;
+            if (win->sinks > 0 && all > 2.0 * tk && !sinks_apart) {
                 sink_tiles = std::min<int64_t>((win->sinks + DkvCfg::BMK - 1) / DkvCfg::BMK, (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK);
-                // (to no longer than the others, and further while there are SMs without a CTA: B2 Hq12 Hkv4 S921 d64 44 us a
-                // launch in four, SINKS8 in eight)
+                // to no longer than the others, and further while there are SMs without a CTA
                 const int64_t ctas = sink_tiles * d->batch * d->kv_heads * DkvCfg::ZS;
                 while (split_sinks < 8 && (all / split_sinks > tk || ctas * split_sinks * 2 <= (int64_t)DkvCfg::CTAS_PER_SM * sms)) split_sinks *= 2;
             }
@@ -786,6 +819,12 @@ int launch_bwd(const tx_sdpa_bwd_desc *d, cudaStream_t st, int *status, const __
         // query heads
         const int64_t slabs = d->batch * d->kv_heads, items = (d->seq_k + DkvCfg::BMK - 1) / DkvCfg::BMK - sink_tiles;
         const int64_t ratio = d->q_heads / d->kv_heads;
+        if constexpr (D <= 128)
+            if (sinks_apart) {
+                if (int rc = launch_sink_grads<txb::SinkGradCfg<D>>(d, st, dout_h, delta, prepared, *win)) return rc;
+                p.apart_k = p.win.sinks;
+                p.win.sinks = 0;
+            }
         if (sink_tiles > 0) {
             txb::BwdParams ps = p;
             ps.group_k = 1; ps.items_k = (int)sink_tiles; ps.slabs_k = (int)slabs; ps.split_k = split_sinks;

@@ -57,10 +57,11 @@ struct BwdParams {
     // item's tiles z, z + split, z + 2 split ... and the cluster adds the partial gradients in rank order.
     int split_q, split_k;
     // WINDOW instantiations (window.cuh).  first_k: key tile of the dK/dV launch's item 0 (its slabs have items_k tiles from
-    // there on); early_k: the launch behind this one reads nothing of it and may start beside it.
+    // there on); early_k: the launch behind this one reads nothing of it and may start beside it; apart_k: so many first keys
+    // are sinks whose gradients another kernel writes.
     WindowRule win;
     int grads_f16 = 0;        // dq, dk, dv are fp16
-    int first_k = 0, early_k = 0;
+    int first_k = 0, early_k = 0, apart_k = 0;
 };
 
 // ------------------------------------------------------------------ result
@@ -90,10 +91,10 @@ __device__ __forceinline__ void stage_grad32(uint32_t tile, uint32_t taddr, int 
 }
 
 // This CTA's share of the tile's rows: summed over the cluster's CTAs in rank order, written to dst[row * ld + column].
-// `fill` stands in for the sum where no CTA of the item had anything to walk.
+// `fill` stands in for the sum where no CTA of the item had anything to walk.  Rows in front of `first` stay as they were.
 template <int W, int THREADS>
 __device__ __forceinline__ void store_grad(const uint8_t *tile, float *dst, int64_t ld, int rows_ok, int rank, int split,
-                                           bool filled, float fill, int tid)
+                                           bool filled, float fill, int tid, int first = 0)
 {
     namespace cg = cooperative_groups;
     constexpr int C = W / 4;
@@ -103,7 +104,7 @@ __device__ __forceinline__ void store_grad(const uint8_t *tile, float *dst, int6
 #pragma unroll 8
         for (int n = 0; n < (N + THREADS - 1) / THREADS; ++n) {
             const int i = n * THREADS + tid, r = i / C, c = i % C;
-            if (i < N && r < rows_ok)
+            if (i < N && r < rows_ok && r >= first)
                 *reinterpret_cast<float4 *>(dst + (int64_t)r * ld + c * 4) =
                     *reinterpret_cast<const float4 *>(tile + grad_chunk<W>(r, c));
         }
@@ -126,14 +127,14 @@ __device__ __forceinline__ void store_grad(const uint8_t *tile, float *dst, int6
             for (int z = 1; z < 8; ++z)
                 if (z < split) { v.x += part[z].x; v.y += part[z].y; v.z += part[z].z; v.w += part[z].w; }
         }
-        *reinterpret_cast<float4 *>(dst + (int64_t)r * ld + c * 4) = v;
+        if (r >= first) *reinterpret_cast<float4 *>(dst + (int64_t)r * ld + c * 4) = v;
     }
 }
 
 // store_grad into fp16 (saturating at nothing: a gradient beyond fp16's range becomes infinite, as a cast would make it)
 template <int W, int THREADS>
 __device__ __forceinline__ void store_grad_half(const uint8_t *tile, __half *dst, int64_t ld, int rows_ok, int rank, int split,
-                                                bool filled, int tid)
+                                                bool filled, int tid, int first = 0)
 {
     namespace cg = cooperative_groups;
     constexpr int C = W / 8;
@@ -159,7 +160,7 @@ __device__ __forceinline__ void store_grad_half(const uint8_t *tile, __half *dst
                     if (z < split) { v[e].x += part[z].x; v[e].y += part[z].y; v[e].z += part[z].z; v[e].w += part[z].w; }
             }
         }
-        *reinterpret_cast<uint4 *>(dst + (int64_t)r * ld + c * 8) =
+        if (r >= first) *reinterpret_cast<uint4 *>(dst + (int64_t)r * ld + c * 8) =
             make_uint4(ptx::pack_half2(v[0].x, v[0].y), ptx::pack_half2(v[0].z, v[0].w), ptx::pack_half2(v[1].x, v[1].y), ptx::pack_half2(v[1].z, v[1].w));
     }
 }
@@ -970,12 +971,13 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         // all, where the forward rows are 0/0 and the reference's rule propagates NaN to every gradient
         const float fill = kv_limit == 0 && !Cfg::WINDOW ? __int_as_float(0x7fc00000) : 0.f;
         const size_t gbase = ((size_t)kvh * p.Sk + key0) * D + col0;
+        const int first = Cfg::WINDOW ? p.apart_k - key0 : 0;
         if (Cfg::WINDOW && p.grads_f16) {
-            store_grad_half<DA, Cfg::THREADS>(smem, reinterpret_cast<__half *>(p.dk) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid);
-            store_grad_half<DA, Cfg::THREADS>(smem + BMK * DA * 4, reinterpret_cast<__half *>(p.dv) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid);
+            store_grad_half<DA, Cfg::THREADS>(smem, reinterpret_cast<__half *>(p.dk) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid, first);
+            store_grad_half<DA, Cfg::THREADS>(smem + BMK * DA * 4, reinterpret_cast<__half *>(p.dv) + gbase, D, p.Sk - key0, rank, split, n_all == 0, tid, first);
         } else {
-        store_grad<DA, Cfg::THREADS>(smem, p.dk + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid);
-        store_grad<DA, Cfg::THREADS>(smem + BMK * DA * 4, p.dv + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid);
+            store_grad<DA, Cfg::THREADS>(smem, p.dk + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid, first);
+            store_grad<DA, Cfg::THREADS>(smem + BMK * DA * 4, p.dv + gbase, D, p.Sk - key0, rank, split, n_all == 0, fill, tid, first);
         }
     } else {
         for (int i = 0; i < 64; ++i) __nanosleep(2000);

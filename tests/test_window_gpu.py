@@ -179,6 +179,33 @@ def test_gradients(case, d):
                 assert not a[n][:, ~see.any(1 if name == "q" else 0)].any(), name
 
 
+SINKS = [
+    # B, Hq, Hkv, Sq, Sk, window, sinks, lens, align: the sinks' tiles are seen by many more rows than the others
+    (1, 4, 2, 1200, 1200, 64, 17, None, "start"),
+    (2, 3, 1, 700, 700, 50, 64, [700, 9], "start"),           # fewer keys than sinks
+    (1, 2, 1, 1200, 1200, 64, 65, None, "start"),
+    (1, 6, 2, 601, 30, 8, 20, None, "start"),                 # rows far behind the last key
+    (1, 2, 2, 500, 900, 40, 5, [800], "end"),
+    (2, 2, 2, 500, 700, 40, 5, [700, 300], "end"),            # rows in front of the first key
+]
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("case", range(len(SINKS)))
+def test_gradients_of_sinks(case, d):
+    """As test_gradients, the norm taken over the sinks' rows alone, then over the others."""
+    B, Hq, Hkv, Sq, Sk, window, sinks, lens, align = SINKS[case]
+    q, k, v = (x.astype(np.float16) for x in (seeded(case, B, Hq, Sq, d), seeded(50 + case, B, Hkv, Sk, d), seeded(90 + case, B, Hkv, Sk, d)))
+    g, full = seeded(7, B, Hq, Sq, d), lens or [Sk] * B
+    want = window_oracle.backward(q, k, v, g, full, window, sinks, align)
+    _, got = gradients(q, k, v, g, window, sinks, lens, align)
+    for name, a, b in zip("qkv", got, want):
+        assert np.isfinite(a).all(), name
+        for part in ((a, b),) if name == "q" else ((a[:, :, :sinks], b[:, :, :sinks]), (a[:, :, sinks:], b[:, :, sinks:])):
+            norm = np.linalg.norm(part[1])
+            assert np.linalg.norm(part[0] - part[1]) <= 2.0 ** -8 * norm, (name, np.linalg.norm(part[0] - part[1]) / max(norm, 1e-30))
+
+
 def test_what_lies_behind_the_last_key_has_no_part_in_gradients():
     for d in (64, 128, 256):
         q, k, v = (seeded(i, 2, 2, 400, d).astype(np.float16) for i in range(3))
