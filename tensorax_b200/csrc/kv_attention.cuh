@@ -42,6 +42,7 @@ struct KvAttnParams {
     const int32_t *q_lens;     // optional [batch]: nodes of each sequence (none: all)
     const uint64_t *tree;      // optional [batch, tokens]: what a node sees of the nodes (none: node t sees 0 .. t)
     int *status;
+    int most_keys;             // what a page table can hold
     int tokens, group;         // group = Hq / Hkv
     int row_parts;             // CTAs (per split) that share the rows of a head, MR each
     int window, sinks;         // window 0: no window
@@ -121,6 +122,14 @@ __device__ __forceinline__ void kv_pairs(uint32_t a, uint32_t b, uint32_t *out)
     kv_halves<FMT>(hi, out[2], out[3]);
 }
 
+// Keys of sequence b.  More than its page table can hold is an error, and not walked.
+__device__ __forceinline__ int kv_length(const KvAttnParams &p, int b, bool &beyond)
+{
+    const int len = p.kv_lens[b];
+    beyond = len > p.most_keys;
+    return max(0, min(len, p.most_keys));
+}
+
 // Weights are kept at 2^kKvShift times what they are: the row's largest then leaves fp16 smaller ones room below (2^-30 of
 // it) and room above for a maximum that has grown by less than 2^kKvLazy since the last rescale.
 constexpr float kKvShift = 6.f, kKvLazy = 8.f;
@@ -146,12 +155,23 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = lane >> 2, t4 = lane & 3;                       // row / column and quarter of the operand layouts
 
+    if (tid == 0) {
+        *bad = 0;
+        *abort_flag = 0;
+        for (int i = 0; i < Cfg::WARPS * NS; ++i) ptx::mbar_init(sbase + Cfg::OFF_BAR + 8 * i, 1);
+        ptx::fence_mbar_init();
+    }
+    // What is in front of this launch in the stream may still run up to here; the loads whose address does not come from one
+    // behind it are plain, since __ldg's may be moved across (a step of 13 tokens over 1500 keys, alone on the chip, again and again: 14.3 us without, 13.0 us).
+    ptx::grid_wait();
     const int item = (int)blockIdx.x / splits;
     const int kvh = item / p.row_parts, row0 = (item % p.row_parts) * MR;    // b * Hkv + h, first row of this part
     const int b = kvh / p.pages.Hkv, h = kvh - b * p.pages.Hkv;
     const int rows = p.group * p.tokens;
-    const int len = max(__ldg(p.kv_lens + b), 0);
-    const int nodes = min(p.q_lens ? min(max(__ldg(p.q_lens + b), 0), p.tokens) : p.tokens, len);
+    bool beyond;
+    const int len = kv_length(p, b, beyond);
+    if (beyond && tid == 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
+    const int nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
     const int ctx = len - nodes;
     // Visible keys as one range of numbers: the sinks in front of the window, then the keys from the window of the shallowest
     // node on, both in whole sixteens.  Number c stands for key c, or c + skip behind the sinks.
@@ -166,15 +186,10 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int share = ((n_vis + splits - 1) / splits + KT - 1) / KT * KT;
     const int c_from = min(split * share, n_vis), c_to = min(c_from + share, n_vis);
 
-    if (tid == 0) {
-        *bad = 0;
-        *abort_flag = *reinterpret_cast<volatile int *>(p.status) != 0 ? 1 : 0;
-        for (int i = 0; i < Cfg::WARPS * NS; ++i) ptx::mbar_init(sbase + Cfg::OFF_BAR + 8 * i, 1);
-        ptx::fence_mbar_init();
-    }
+    if (tid == 0 && *reinterpret_cast<volatile int *>(p.status) != 0) *abort_flag = 1;
     for (int r = tid; r < MR; r += Cfg::THREADS) {           // a row beyond the last repeats it and is never written
         const int t = min(row0 + r, rows - 1) % p.tokens;
-        const uint64_t word = p.tree ? __ldg(p.tree + (int64_t)b * p.tokens + t) : ~0ull >> (63 - t);
+        const uint64_t word = p.tree ? p.tree[(int64_t)b * p.tokens + t] : ~0ull >> (63 - t);
         words[r] = word;
         lows[r] = p.window > 0 ? ctx + max(__popcll(word), 1) - p.window : 0;
     }
@@ -247,7 +262,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(q + 16 * (t4 + 4 * c)) + half);
+                    const uint4 u = reinterpret_cast<const uint4 *>(q + 16 * (t4 + 4 * c))[half];
                     const int step = 4 * c + 2 * half;
                     if constexpr (Cfg::Q_IN_REGS) {
                         qr[step][r] = make_uint2(u.x, u.y);
@@ -265,7 +280,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float4 f = __ldg(reinterpret_cast<const float4 *>(q + 16 * (t4 + 4 * c)) + e);
+                    const float4 f = reinterpret_cast<const float4 *>(q + 16 * (t4 + 4 * c))[e];
                     x[16 * c + 4 * e] = f.x; x[16 * c + 4 * e + 1] = f.y; x[16 * c + 4 * e + 2] = f.z; x[16 * c + 4 * e + 3] = f.w;
                 }
 #pragma unroll

@@ -121,13 +121,15 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
     const int split = (int)cluster.block_rank(), splits = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    ptx::grid_wait();            // as in kv_attention_kernel
     // work item and keys, numbered as in kv_attention_kernel
     const int item = (int)blockIdx.x / splits;
     const int kvh = item / p.row_parts, row0 = (item % p.row_parts) * MR;
     const int b = kvh / p.pages.Hkv, h = kvh - b * p.pages.Hkv;
     const int rows = p.group * p.tokens;
-    const int len = max(__ldg(p.kv_lens + b), 0);
-    const int nodes = min(p.q_lens ? min(max(__ldg(p.q_lens + b), 0), p.tokens) : p.tokens, len);
+    bool beyond = false;
+    const int len = kv_length(p, b, beyond);
+    const int nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
     const int ctx = len - nodes;
     int first = 0, s_end = 0;
     if (p.window > 0) {
@@ -143,7 +145,8 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
     const int n1 = live1 ? n_tiles : 0;
 
     if (tid == 0) {
-        *bad = 0;
+        *bad = beyond ? 1 : 0;
+        if (beyond) ptx::report(p.status, KV_ERR_PAGE);
         *abort_flag = 0;
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(k_ready + 8 * t, Cfg::CONVERTERS);     // one arrival per converter warp
@@ -167,12 +170,20 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         ptx::tmem_relinquish();
     }
     // Q: rows of this part are one run of memory; rows behind the last are zero
-#pragma unroll 4
-    for (int i = tid; i < MR * (D / 8); i += Cfg::THREADS) {
-        const int r = i / (D / 8), c = i % (D / 8);
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (row0 + r < rows) x = __ldg(reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.q) + ((int64_t)kvh * rows + row0 + r) * D) + c);
-        ptx::st_shared_v4(q_s + (r / BM) * Cfg::Q_TILE + (c >> 3) * (BM * 128) + (r % BM) * 128 + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+    constexpr int Q_LOADS = MR * (D / 8) / Cfg::THREADS;
+    static_assert(MR * (D / 8) % Cfg::THREADS == 0, "whole turns");
+    uint4 q_in[Q_LOADS];
+#pragma unroll
+    for (int n = 0; n < Q_LOADS; ++n) {
+        const int i = n * Cfg::THREADS + tid, r = i / (D / 8), c = i % (D / 8);
+        q_in[n] = make_uint4(0u, 0u, 0u, 0u);
+        if (row0 + r < rows) q_in[n] = reinterpret_cast<const uint4 *>(static_cast<const __half *>(p.q) + ((int64_t)kvh * rows + row0 + r) * D)[c];
+    }
+#pragma unroll
+    for (int n = 0; n < Q_LOADS; ++n) {
+        const int i = n * Cfg::THREADS + tid, r = i / (D / 8), c = i % (D / 8);
+        ptx::st_shared_v4(q_s + (r / BM) * Cfg::Q_TILE + (c >> 3) * (BM * 128) + (r % BM) * 128 + (((c & 7) ^ (r & 7)) << 4), q_in[n].x, q_in[n].y,
+                          q_in[n].z, q_in[n].w);
     }
     ptx::fence_proxy_async_smem();
     ptx::tc_fence_before_sync();
@@ -376,7 +387,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t t_s = tmem + lane_base + (t ? Cfg::COL_S1 : Cfg::COL_S0), t_o = tmem + lane_base + (t ? Cfg::COL_O1 : Cfg::COL_O0);
         const int node = min(row, rows - 1) % p.tokens;
-        uint64_t word = p.tree ? __ldg(p.tree + (int64_t)b * p.tokens + node) : ~0ull >> (63 - node);
+        uint64_t word = p.tree ? p.tree[(int64_t)b * p.tokens + node] : ~0ull >> (63 - node);
         const int low = p.window > 0 ? ctx + max(__popcll(word), 1) - p.window : 0;
         if (nodes < 64) word &= (1ull << nodes) - 1;
         float m_used = -1.0e30f, l = 0.f, vref = 1.f;             // a finite stand-in for "no key seen yet"

@@ -131,16 +131,19 @@ template <class... Params, class... Args>
 int launch_cluster(void (*kernel)(Params...), int64_t ctas, int cluster, int threads, size_t smem, void *stream, const Args &...args)
 {
     if (ctas > 0x7fffffffLL) return fail(TX_ERR_UNSUPPORTED, "K/V cache attention: more than 2^31 work items");
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = (unsigned)cluster; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    // (the kernels wait for what is in front of them in the stream before they read anything)
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cluster; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     TX_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     txb::api::launched();
     return TX_OK;
@@ -239,6 +242,7 @@ int tx_kv_cache_attention(const tx_kv_attention_desc *d)
     p.kv_lens = d->kv_lens; p.q_lens = d->q_lens; p.tree = d->tree;
     p.tokens = (int)d->tokens; p.group = (int)(d->q_heads / d->cache.kv_heads);
     p.row_parts = 0;
+    p.most_keys = (int)(d->table_len * d->cache.page_size);
     // a window longer than any sequence is none
     p.window = (int)std::min<int64_t>(d->window, 0x7fffffffLL); p.sinks = (int)std::min<int64_t>(d->sinks, 0x7fffffffLL);
     p.out_f16 = (d->flags & TX_SDPA_OUT_F16) ? 1 : 0;

@@ -122,6 +122,20 @@ def test_what_does_not_exist_is_reported_and_left_out(what):
     _lib.check(_lib.load().tx_sdpa_finish(None))
 
 
+@pytest.mark.parametrize("length", [41, 2 ** 31 - 1])
+@pytest.mark.parametrize("heads", [1, 40])
+def test_more_keys_than_the_page_table_holds(heads, length):
+    """Reported, the sequence's rows NaN (the failure is the whole call's: another sequence may or may not have its rows)."""
+    B, H, d, page = 2, 1, 64, 16
+    cache, table, _ = filled(3, B, H, 32, d, page, "int8")
+    q = tensor(seeded(4, B, H * heads, 2, d).astype(np.float16))
+    out = cache.attend(q, table, [length, 32], sync=False)
+    with pytest.raises(RuntimeError, match="does not exist"):
+        _lib.check(_lib.load().tx_sdpa_finish(None))
+    assert np.isnan(out.numpy()[0]).all()
+    assert np.isfinite(cache.attend(q, table, [32, 32]).numpy()).all()
+
+
 # ------------------------------------------------------------------ attention
 def filled(seed, B, H, S, d, page, fmt, spread=0.5):
     """A cache of S tokens per sequence, its page table, and the values it holds [2][B, H, S, d]."""
