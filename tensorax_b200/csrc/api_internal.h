@@ -4,6 +4,9 @@
 
 #include <cstdint>
 
+#include "../../include/tensorax_b200.h"
+#include "kv_lens.cuh"
+
 namespace txb {
 
 enum : int { KV_ERR_PAGE = 51 };      // failure word: see kv_cache.cuh
@@ -18,6 +21,9 @@ int current_device(int *dev);
 // `rows` rows of d one-byte codes as 128-byte lines, copied sixteen rows at a time with a 128-byte swizzle
 int map_of_codes(CUtensorMap *m, const void *base, int64_t rows, int64_t d);
 void launched();                     // counts one kernel launch
+// kv_cache_api.cu: a decoding step of fp16 rows with a window over plain K and V, by the kernel of the cache's attention
+bool window_step_fits(const tx_sdpa_desc *d);
+int window_step(const tx_sdpa_desc *d, const KvLens &lens, int window, int sinks, int align_end, int *status);
 
 }  // namespace api
 }  // namespace txb

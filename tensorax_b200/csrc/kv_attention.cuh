@@ -26,13 +26,22 @@
 //
 // fp32 queries: Q (scaled by a power of two per row) and P are carried as two fp16 numbers each, and the products of a
 // stage are added to O in fp32 instead of in the matrix unit, whose sums are cut off rather than rounded.
+//
+// The same kernel takes decoding steps of the windowed attention over plain fp16 keys (KV_PLAIN), weights as two numbers each as
+// everywhere in decoding steps: B8 Hq32 Hkv8 d128, window 2048, four sinks, 16.9 us, 27.7 by the kernel of sdpa_decode.cuh, whose
+// products are fp32 FMAs.
 #pragma once
 #include <cfloat>
 #include <cooperative_groups.h>
 
 #include "kv_cache.cuh"
+#include "kv_lens.cuh"
 
 namespace txb {
+
+// Not a cache's format: K and V as they are, [B, Hkv, Sk, D] fp16, the rows of a window (window.cuh) at its keys.  A page is a
+// head's keys, and there are no scales; sixteen keys at the end of one head may be the next one's (masked, V's zeroed).
+constexpr int KV_PLAIN = 2;
 
 struct KvAttnParams {
     KvPages pages;
@@ -50,23 +59,28 @@ struct KvAttnParams {
     float scale_log2;          // log2(e) / sqrt(D)
 };
 
+struct KvPlainParams : KvAttnParams {
+    KvLens lens;
+    int Sk, align_end;
+};
+
 enum : int { KV_ERR_ROWS = 54 };
 
-// Byte offset of 16-byte chunk c of key r in a stage's K or V tile: 128-byte lines, their chunks swizzled by the copy
-template <int D>
+// Byte offset of 16-byte chunk c of key r, B bytes long, in a stage's K or V tile: 128-byte lines, their chunks swizzled by the copy
+template <int B>
 __device__ __forceinline__ uint32_t kv_at(int r, int c)
 {
-    const int at = r * (D / 16) + c, line = at >> 3;
+    const int at = r * (B / 16) + c, line = at >> 3;
     return (uint32_t)(line * 128 + (((at & 7) ^ (line & 7)) << 4));
 }
 // Which of eight keys is row n of the products, as 3 bits each.  K is read by eight lanes at a time, chunks t (+ 4 i) of rows
 // 2 t', 2 t' + 1: the two keys must lie in different halves of their lines.  V by eight lanes, chunks n, n + 1 of rows 0, 2, 4, 6
-// or 1, 3, 5, 7 (at D = 64 by sixteen, halves of two chunks): four keys whose swizzles take these to different quarters.
-template <int D>
+// or 1, 3, 5, 7 (at 64 bytes by sixteen, halves of two chunks): four keys whose swizzles take these to different quarters.
+template <int B>
 __device__ __forceinline__ int kv_key(int n)
 {
     constexpr int order[3][8] = {{0, 3, 4, 7, 1, 2, 5, 6}, {0, 5, 2, 7, 4, 1, 6, 3}, {0, 6, 1, 7, 2, 4, 3, 5}};
-    constexpr int w = D == 64 ? 0 : D == 128 ? 1 : 2;
+    constexpr int w = B == 64 ? 0 : B == 128 ? 1 : 2;
     constexpr uint32_t bits = order[w][0] | order[w][1] << 3 | order[w][2] << 6 | order[w][3] << 9 | order[w][4] << 12 |
                               order[w][5] << 15 | order[w][6] << 18 | order[w][7] << 21;
     return bits >> (3 * n) & 7;
@@ -76,12 +90,14 @@ template <typename TQ_, int FMT_, int D_, int NR_, int WARPS_, int KW_, int NS_,
 struct KvAttnCfg {
     using TQ = TQ_;
     static constexpr int FMT = FMT_, D = D_, NR = NR_, WARPS = WARPS_, KW = KW_, NS = NS_, CTAS_PER_SM = CTAS_PER_SM_;
-    static constexpr bool F32 = sizeof(TQ_) == 4;
+    static constexpr bool F32 = sizeof(TQ_) == 4, PLAIN = FMT == KV_PLAIN, P2 = F32 || PLAIN;
+    using Params = std::conditional_t<PLAIN, KvPlainParams, KvAttnParams>;
+    static constexpr int ROW = PLAIN ? 2 * D : D;                         // bytes of a key
     static constexpr bool Q_IN_REGS = !F32 && D * NR <= 256;
     static constexpr int MR = 8 * NR, THREADS = 32 * WARPS, KT = WARPS * KW;
-    static constexpr uint32_t TILE = KW * D, STAGE = 2 * TILE;            // K, V of a step of one warp
+    static constexpr uint32_t TILE = KW * ROW, STAGE = 2 * TILE;            // K, V of a step of one warp
     static constexpr uint32_t OFF_SCALES = WARPS * NS * STAGE;            // [WARPS][NS][K, V][KW]
-    static constexpr uint32_t RING = OFF_SCALES + WARPS * NS * KW * 8;
+    static constexpr uint32_t RING = OFF_SCALES + (PLAIN ? 0 : WARPS * NS * KW * 8);
     static constexpr uint32_t MERGE = WARPS * MR * D * 4;                 // partial O of every warp, over the drained rings
     static constexpr uint32_t OFF_Q = RING > MERGE ? RING : MERGE;
     static constexpr uint32_t Q_BYTES = Q_IN_REGS ? 0 : MR * D * 2 * (F32 ? 2 : 1);   // operand order, hi (and lo)
@@ -93,6 +109,7 @@ struct KvAttnCfg {
     static constexpr uint32_t SMEM = OFF_FLAG + 16;
     static constexpr int MAX_SPLITS = 16;
     static_assert(D == 64 || D == 128 || D == 256, "head dims");
+    static_assert(!PLAIN || (!F32 && D <= 128), "plain keys: fp16, up to 256 bytes");
     static_assert(KW == 16 || KW == 32, "step shapes");
     static_assert(SMEM <= 232448 && (CTAS_PER_SM * (SMEM + 1024) <= 233472), "shared memory of an SM");
 };
@@ -137,12 +154,12 @@ constexpr float kKvShift = 6.f, kKvLazy = 8.f;
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM)
 kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                    const __grid_constant__ KvAttnParams p)
+                    const __grid_constant__ typename Cfg::Params p)
 {
     using TQ = typename Cfg::TQ;
-    constexpr int D = Cfg::D, NR = Cfg::NR, KW = Cfg::KW, KT = Cfg::KT, NS = Cfg::NS, FMT = Cfg::FMT, MR = Cfg::MR;
+    constexpr int D = Cfg::D, ROW = Cfg::ROW, NR = Cfg::NR, KW = Cfg::KW, KT = Cfg::KT, NS = Cfg::NS, FMT = Cfg::FMT, MR = Cfg::MR;
     constexpr int NG = KW / 16, KSTEPS = D / 16, OT = D / 16;
-    constexpr bool F32 = Cfg::F32;
+    constexpr bool F32 = Cfg::F32, PLAIN = Cfg::PLAIN, P2 = Cfg::P2;
     namespace cg = cooperative_groups;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t sbase = ptx::smem_u32(smem);
@@ -168,11 +185,19 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int kvh = item / p.row_parts, row0 = (item % p.row_parts) * MR;    // b * Hkv + h, first row of this part
     const int b = kvh / p.pages.Hkv, h = kvh - b * p.pages.Hkv;
     const int rows = p.group * p.tokens;
-    bool beyond;
-    const int len = kv_length(p, b, beyond);
-    if (beyond && tid == 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
-    const int nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
-    const int ctx = len - nodes;
+    int len, nodes, ctx;                                          // keys of the sequence, rows of a head, position of the first
+    if constexpr (PLAIN) {
+        len = p.lens.limit(b, p.Sk);
+        nodes = p.tokens;
+        ctx = p.align_end ? len - p.tokens : 0;
+        len = max(0, min(len, ctx + p.tokens));
+    } else {
+        bool beyond;
+        len = kv_length(p, b, beyond);
+        if (beyond && tid == 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
+        nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
+        ctx = len - nodes;
+    }
     // Visible keys as one range of numbers: the sinks in front of the window, then the keys from the window of the shallowest
     // node on, both in whole sixteens.  Number c stands for key c, or c + skip behind the sinks.
     int first = 0, s_end = 0;
@@ -189,6 +214,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (tid == 0 && *reinterpret_cast<volatile int *>(p.status) != 0) *abort_flag = 1;
     for (int r = tid; r < MR; r += Cfg::THREADS) {           // a row beyond the last repeats it and is never written
         const int t = min(row0 + r, rows - 1) % p.tokens;
+        if constexpr (PLAIN) { lows[r] = ctx + t + 1 - p.window; continue; }
         const uint64_t word = p.tree ? p.tree[(int64_t)b * p.tokens + t] : ~0ull >> (63 - t);
         words[r] = word;
         lows[r] = p.window > 0 ? ctx + max(__popcll(word), 1) - p.window : 0;
@@ -210,6 +236,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         return c >= c_to || lane >= NG ? -1 : c < s_end ? c : c + skip;
     };
     auto look_up = [&](int j) {
+        if constexpr (PLAIN) return;
         const int pos = j < n_steps ? position(j) : -1;
         page = -1;
         if (pos >= 0 && (pos >> p.pages.page_shift) < p.pages.table_len)
@@ -217,19 +244,22 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     };
     auto request = [&](int j) {                                   // step j, into the place that the warp is done with
         const int slot = j % NS, pos = position(j);
-        const bool there = page >= 0 && page < p.pages.pages && pos >= 0;
-        const int64_t row = ((((int64_t)page * p.pages.Hkv + h) << p.pages.page_shift)) + (pos & ((1 << p.pages.page_shift) - 1));
+        const bool there = pos >= 0 && (PLAIN || (page >= 0 && page < p.pages.pages));
+        int64_t row;
+        if constexpr (PLAIN) row = (int64_t)kvh * p.Sk + pos;
+        else row = ((((int64_t)page * p.pages.Hkv + h) << p.pages.page_shift)) + (pos & ((1 << p.pages.page_shift) - 1));
         if (!there && pos >= 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
         look_up(j + 1);
         const uint32_t n_there = NG == 1 ? (there ? 1 : 0) : __popc(__ballot_sync(0xffffffffu, there));
-        if (lane == 0) ptx::mbar_arrive_expect_tx(full + 8 * slot, n_there * (16 * 2 * D));
+        if (lane == 0) ptx::mbar_arrive_expect_tx(full + 8 * slot, n_there * (16 * 2 * ROW));
         if (NG > 1) __syncwarp();
         if (there) {
-            const uint32_t k_s = ring + slot * Cfg::STAGE + lane * 16 * D;
-            const int line = (int)(row * D / 128);
+            const uint32_t k_s = ring + slot * Cfg::STAGE + lane * 16 * ROW;
+            const int line = (int)(row * ROW / 128);
             ptx::tma_load_3d(k_s, &tm_k, full + 8 * slot, 0, line, 0);
             ptx::tma_load_3d(k_s + Cfg::TILE, &tm_v, full + 8 * slot, 0, line, 0);
         }
+        if constexpr (PLAIN) return;
         // a scale a lane: bulk copies of 64 bytes cost the copy engine as much as the codes'
 #pragma unroll
         for (int g = 0; g < NG; ++g) {
@@ -257,7 +287,15 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (int r = 0; r < NR; ++r) {
         const int row = min(row0 + 8 * r + n, rows - 1);
         const TQ *q = static_cast<const TQ *>(p.q) + ((int64_t)kvh * rows + row) * D;
-        if constexpr (!F32) {
+        if constexpr (PLAIN) {
+            // a lane's chunk is eight elements here, its share of two steps
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(q + 8 * (t4 + 4 * c));
+                qr[2 * c][r] = make_uint2(u.x, u.y);
+                qr[2 * c + 1][r] = make_uint2(u.z, u.w);
+            }
+        } else if constexpr (!F32) {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -324,19 +362,30 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     for (int r = 0; r < NR; ++r)
 #pragma unroll
         for (int i = 0; i < 2; ++i) { m[r][i] = -FLT_MAX; l[r][i] = 0.f; }
-    uint32_t ref = 1u << 23;                                      // bits of the power of two that weights are divided by
-    float inv_ref = __int_as_float(253 << 23);
+    uint32_t ref = PLAIN ? 127u << 23 : 1u << 23;                 // bits of the power of two that weights are divided by
+    float inv_ref = __int_as_float(PLAIN ? 127 << 23 : 253 << 23);
 
-    const int key_n = kv_key<D>(n), key_t[2] = {kv_key<D>(2 * t4), kv_key<D>(2 * t4 + 1)};    // K's row and V's of this lane
+    const int key_n = kv_key<ROW>(n), key_t[2] = {kv_key<ROW>(2 * t4), kv_key<ROW>(2 * t4 + 1)};    // K's row and V's of this lane
     auto step = [&](int j) {
         const uint8_t *k_s = smem + (warp * NS + j % NS) * Cfg::STAGE, *v_s = k_s + Cfg::TILE;
         const float *ksc = reinterpret_cast<const float *>(smem + Cfg::OFF_SCALES + (warp * NS + j % NS) * KW * 8), *vsc = ksc + KW;
         const int c0 = c_from + j * KT + warp * KW;               // number of the step's first key
+        const int key0 = c0 < s_end ? c0 : c0 + skip, key1 = c0 + KW - 1 < s_end ? c0 + KW - 1 : c0 + KW - 1 + skip;
+        auto clear = [&](int i) {                                 // chunk i of V's stage
+            *reinterpret_cast<uint4 *>(const_cast<uint8_t *>(v_s) + kv_at<ROW>(i / (ROW / 16), i % (ROW / 16))) = make_uint4(0u, 0u, 0u, 0u);
+        };
+        if (PLAIN && key0 < ctx + 1 - p.window && key1 >= p.sinks) {
+            // between the sinks and the first row's window: keys that no row sees may hold anything, NaN too (codes are finite)
+            for (int i = lane; i < KW * (ROW / 16); i += 32) {
+                const int c = c0 + i / (ROW / 16), key = c < s_end ? c : c + skip;
+                if (key < ctx + 1 - p.window && key >= p.sinks) clear(i);
+            }
+            __syncwarp();
+            ptx::fence_proxy_async_smem();
+        }
         if (c0 + KW > c_to) {
             // behind the last key: whatever the page or the ring held there, times a weight of zero, must be zero
-            const int from = c_to - c0;
-            for (int i = lane; i < (KW - from) * (D / 16); i += 32)
-                *reinterpret_cast<uint4 *>(const_cast<uint8_t *>(v_s) + kv_at<D>(from + i / (D / 16), i % (D / 16))) = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = (c_to - c0) * (ROW / 16) + lane; i < KW * (ROW / 16); i += 32) clear(i);
             __syncwarp();
             ptx::fence_proxy_async_smem();                        // before the copy that refills the stage
         }
@@ -345,27 +394,33 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
         for (int i = 0; i < NG * NR * 4; ++i) s[i / (NR * 4)][i / 4 % NR][i % 4] = 0.f;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
+        for (int c = 0; c < ROW / 64; ++c) {
             uint32_t kw[NG][2][4];
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const uint4 x = *reinterpret_cast<const uint4 *>(k_s + kv_at<D>(16 * g + 8 * u + key_n, t4 + 4 * c));
+                    const uint4 x = *reinterpret_cast<const uint4 *>(k_s + kv_at<ROW>(16 * g + 8 * u + key_n, t4 + 4 * c));
                     kw[g][u][0] = x.x; kw[g][u][1] = x.y; kw[g][u][2] = x.z; kw[g][u][3] = x.w;
                 }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < (PLAIN ? 2 : 4); ++e) {
+                constexpr int STEPS = PLAIN ? 2 : 4;              // of a chunk
                 uint32_t a[NG][4];
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    kv_halves<FMT>(kw[g][0][e], a[g][0], a[g][2]);
-                    kv_halves<FMT>(kw[g][1][e], a[g][1], a[g][3]);
+                    if constexpr (PLAIN) {
+                        a[g][0] = kw[g][0][2 * e]; a[g][2] = kw[g][0][2 * e + 1];
+                        a[g][1] = kw[g][1][2 * e]; a[g][3] = kw[g][1][2 * e + 1];
+                    } else {
+                        kv_halves<FMT>(kw[g][0][e], a[g][0], a[g][2]);
+                        kv_halves<FMT>(kw[g][1][e], a[g][1], a[g][3]);
+                    }
                 }
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     uint2 q;
-                    if constexpr (Cfg::Q_IN_REGS) q = qr[4 * c + e][r];
+                    if constexpr (Cfg::Q_IN_REGS) q = qr[STEPS * c + e][r];
                     else q = q_s[((4 * c + e) * NR + r) * 32 + lane];
 #pragma unroll
                     for (int g = 0; g < NG; ++g) kv_mma(s[g][r], a[g], q.x, q.y);
@@ -378,7 +433,6 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
         }
         // scores in units of log2, masks
-        const int key0 = c0 < s_end ? c0 : c0 + skip, key1 = c0 + KW - 1 < s_end ? c0 + KW - 1 : c0 + KW - 1 + skip;
         const bool need_mask = key1 >= ctx || (key0 < all_see && key1 >= p.sinks);
         float mx[NR][2];
 #pragma unroll
@@ -387,7 +441,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float f = ksc[16 * g + 8 * u + key_n] * (F32 ? 1.f : p.scale_log2);
+                float f = F32 ? 1.f : p.scale_log2;
+                if constexpr (!PLAIN) f *= ksc[16 * g + 8 * u + key_n];
 #pragma unroll
                 for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -399,7 +454,9 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const int row = 8 * r + 2 * t4 + i;
-                            const bool sees = key < ctx ? (key >= lows[row] || key < p.sinks) : (c < c_to && (words[row] >> (key - ctx) & 1));
+                            bool sees;
+                            if constexpr (PLAIN) sees = c < c_to && key < lows[row] + p.window && (key >= lows[row] || key < p.sinks);
+                            else sees = key < ctx ? (key >= lows[row] || key < p.sinks) : (c < c_to && (words[row] >> (key - ctx) & 1));
                             if (!sees) s[g][r][2 * u + i] = -INFINITY;
                         }
                 }
@@ -409,9 +466,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     for (int i = 0; i < 2; ++i) mx[r][i] = fmaxf(mx[r][i], s[g][r][2 * u + i]);
             }
         // the largest scale of the step's values; one that is not finite counts for the rows that see it only
-        float my_vs = lane < KW && c0 + lane < c_to ? vsc[lane] : 0.f;
-        if (!(my_vs < INFINITY)) my_vs = 0.f;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(my_vs));
+        uint32_t top = 0;
+        if constexpr (!PLAIN) {
+            float my_vs = lane < KW && c0 + lane < c_to ? vsc[lane] : 0.f;
+            if (!(my_vs < INFINITY)) my_vs = 0.f;
+            top = __reduce_max_sync(0xffffffffu, __float_as_uint(my_vs));
+        }
         float alpha[NR][2];
         bool rescale = false;
 #pragma unroll
@@ -426,7 +486,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 m[r][i] = next;
                 l[r][i] *= alpha[r][i];
             }
-        if (top > ref) {
+        if (!PLAIN && top > ref) {
             const uint32_t next = min((top + 0x7fffffu) & 0x7f800000u, 253u << 23);
             const float f = __uint_as_float(ref) * __uint_as_float((254u << 23) - next);      // powers of two
             ref = next;
@@ -444,12 +504,12 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     for (int e = 0; e < 4; ++e) o[d][r][e] *= alpha[r][e & 1];
         }
         // weights, as operands of the second product
-        uint32_t pa[NG][NR][2], pl[F32 ? NG : 1][NR][2];
+        uint32_t pa[NG][NR][2], pl[P2 ? NG : 1][NR][2];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float f = vsc[16 * g + 8 * u + key_n] * inv_ref;
+                const float f = PLAIN ? 1.f : vsc[16 * g + 8 * u + key_n] * inv_ref;
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     float x[2];
@@ -462,7 +522,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     }
                     const uint32_t hi = ptx::pack_half2(x[0], x[1]);
                     pa[g][r][u] = kv_transpose(hi);
-                    if constexpr (F32) {
+                    if constexpr (P2) {
                         const float2 back = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
                         pl[g][r][u] = kv_transpose(ptx::pack_half2(x[0] - back.x, x[1] - back.y));
                     }
@@ -470,19 +530,19 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             }
         // O^T += V^T P^T: the two tiles of a word's four columns at a time
 #pragma unroll
-        for (int c = 0; c < (D + 127) / 128; ++c) {
-            constexpr int WORDS = D == 64 ? 2 : 4;
+        for (int c = 0; c < (ROW + 127) / 128; ++c) {
+            constexpr int WORDS = ROW == 64 ? 2 : 4;
             uint32_t v[NG][4][WORDS];
 #pragma unroll
             for (int g = 0; g < NG; ++g)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const int row = g * 16 + key_t[x & 1] + (x >> 1) * 8;
-                    if constexpr (D == 64) {
-                        const uint2 u = *reinterpret_cast<const uint2 *>(v_s + kv_at<D>(row, n >> 1) + (n & 1) * 8);
+                    if constexpr (ROW == 64) {
+                        const uint2 u = *reinterpret_cast<const uint2 *>(v_s + kv_at<ROW>(row, n >> 1) + (n & 1) * 8);
                         v[g][x][0] = u.x; v[g][x][1] = u.y;
                     } else {
-                        const uint4 u = *reinterpret_cast<const uint4 *>(v_s + kv_at<D>(row, n + 8 * c));
+                        const uint4 u = *reinterpret_cast<const uint4 *>(v_s + kv_at<ROW>(row, n + 8 * c));
                         v[g][x][0] = u.x; v[g][x][1] = u.y; v[g][x][2] = u.z; v[g][x][3] = u.w;
                     }
                 }
@@ -494,19 +554,26 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     for (int e = 0; e < 2 * NR * 4; ++e) part[e / (NR * 4)][e / 4 % NR][e % 4] = 0.f;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    uint32_t a0[4], a1[4];                        // bytes 0 .. 3 of keys 2 t4, 2 t4 + 1 and of keys 8 further
-                    kv_pairs<FMT>(v[g][0][w], v[g][1][w], a0);
-                    kv_pairs<FMT>(v[g][2][w], v[g][3][w], a1);
+                    constexpr int TILES = PLAIN ? 1 : 2;          // of a word's columns
+                    uint32_t a[2][4];
+                    if constexpr (PLAIN) {
+                        a[0][0] = __byte_perm(v[g][0][w], v[g][1][w], 0x5410); a[0][1] = __byte_perm(v[g][0][w], v[g][1][w], 0x7632);
+                        a[0][2] = __byte_perm(v[g][2][w], v[g][3][w], 0x5410); a[0][3] = __byte_perm(v[g][2][w], v[g][3][w], 0x7632);
+                    } else {
+                        uint32_t a0[4], a1[4];                    // bytes 0 .. 3 of keys 2 t4, 2 t4 + 1 and of keys 8 further
+                        kv_pairs<FMT>(v[g][0][w], v[g][1][w], a0);
+                        kv_pairs<FMT>(v[g][2][w], v[g][3][w], a1);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t a[4] = {a0[2 * e], a0[2 * e + 1], a1[2 * e], a1[2 * e + 1]};
+                        for (int e = 0; e < 2; ++e) { a[e][0] = a0[2 * e]; a[e][1] = a0[2 * e + 1]; a[e][2] = a1[2 * e]; a[e][3] = a1[2 * e + 1]; }
+                    }
+#pragma unroll
+                    for (int e = 0; e < TILES; ++e)
 #pragma unroll
                         for (int r = 0; r < NR; ++r) {
-                            float *acc = F32 ? part[F32 ? e : 0][r] : o[c * 8 + w * 2 + e][r];
-                            kv_mma(acc, a, pa[g][r][0], pa[g][r][1]);
-                            if constexpr (F32) kv_mma(acc, a, pl[g][r][0], pl[g][r][1]);
+                            float *acc = F32 ? part[F32 ? e : 0][r] : o[(c * 4 + w) * TILES + e][r];
+                            kv_mma(acc, a[e], pa[g][r][0], pa[g][r][1]);
+                            if constexpr (P2) kv_mma(acc, a[e], pl[g][r][0], pl[g][r][1]);
                         }
-                    }
                 }
                 if constexpr (F32)
 #pragma unroll
@@ -527,7 +594,8 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     if (run && !ok) { *abort_flag = 1; ptx::report(p.status, KV_ERR_ROWS); }
 
     // ------------------------------------------------------------ partial results
-    // o[8 c + i][r][2 u + k]: element 128 c + 16 n + 2 i + u (at D = 64: 8 n + 2 i + u) of row 8 r + 2 t4 + k
+    // o[8 c + i][r][2 u + k]: element 128 c + 16 n + 2 i + u (at D = 64: 8 n + 2 i + u) of row 8 r + 2 t4 + k; plain keys:
+    // o[4 c + i], element 64 c + 8 n + 2 i + u
 #pragma unroll
     for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -537,7 +605,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     kv_copy_wait<0>();
     __syncthreads();                                              // the rings are drained
     {
-        constexpr int RUN = D == 64 ? 8 : 16;
+        constexpr int RUN = D == 64 || PLAIN ? 8 : 16, SPAN = D < 8 * RUN ? D : 8 * RUN;
         const float unit = __uint_as_float(ref);
         float *mine = part + warp * MR * D;
 #pragma unroll
@@ -547,12 +615,13 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 const int row = 8 * r + 2 * t4 + k;
                 if (n == 0) ml[warp * MR + row] = make_float2(m[r][k], l[r][k]);
 #pragma unroll
-                for (int c = 0; c < (D + 127) / 128; ++c)
+                for (int c = 0; c < D / SPAN; ++c)
 #pragma unroll
-                    for (int x = 0; x < RUN / 2; x += 2)
-                        *reinterpret_cast<float4 *>(mine + row * D + 128 * c + RUN * n + 2 * x) =
-                            make_float4(o[8 * c + x][r][k] * unit, o[8 * c + x][r][2 + k] * unit,
-                                        o[8 * c + x + 1][r][k] * unit, o[8 * c + x + 1][r][2 + k] * unit);
+                    for (int x = 0; x < RUN / 2; x += 2) {
+                        const int i = RUN / 2 * c + x;
+                        *reinterpret_cast<float4 *>(mine + row * D + SPAN * c + RUN * n + 2 * x) =
+                            make_float4(o[i][r][k] * unit, o[i][r][2 + k] * unit, o[i + 1][r][k] * unit, o[i + 1][r][2 + k] * unit);
+                    }
             }
     }
     __syncthreads();

@@ -119,12 +119,16 @@ int allow_launch(int smem)
 // CTAs of a cluster that share the keys of an item: as many as one wave holds -- up to eight, or sixteen -- as long as each has
 // a tile of KT of the most keys that the call can see.  B16 Hkv8, 4096 to 8192 keys, d128, a row a head: in two 50.2 us, in three
 // 45.5 (all places of one wave), in four 57.0, in six 49.7.
-int splits_of(const tx_kv_attention_desc *d, int64_t items, int64_t places, int most, int kt)
+int splits_of(int64_t keys, int64_t items, int64_t places, int most, int kt)
 {
-    int64_t keys = d->table_len * d->cache.page_size;
-    if (d->window > 0) keys = std::min(keys, d->window + d->sinks + d->tokens);
     const int64_t splits = std::max<int64_t>(1, std::min({(int64_t)most, places / items, (keys + kt - 1) / kt}));
     return splits >= 16 ? 16 : (int)std::min<int64_t>(splits, 8);
+}
+
+int64_t keys_seen(const tx_kv_attention_desc *d)
+{
+    const int64_t keys = d->table_len * d->cache.page_size;
+    return d->window > 0 ? std::min(keys, std::min<int64_t>(d->window, 0x7fffffff) + std::min<int64_t>(d->sinks, 0x7fffffff) + d->tokens) : keys;
 }
 
 template <class... Params, class... Args>
@@ -157,7 +161,7 @@ int launch_attention_t(txb::KvAttnParams p, const tx_kv_attention_desc *d)
     const int64_t items = d->batch * d->cache.kv_heads * p.row_parts;
     int sms = 0;
     if (int rc = txb::api::sm_count(&sms)) return rc;
-    const int splits = splits_of(d, items, (int64_t)Cfg::CTAS_PER_SM * sms, Cfg::MAX_SPLITS, Cfg::KT);
+    const int splits = splits_of(keys_seen(d), items, (int64_t)Cfg::CTAS_PER_SM * sms, Cfg::MAX_SPLITS, Cfg::KT);
     if (int rc = allow_launch<txb::kv_attention_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
     CUtensorMap tk, tv;
     const int64_t cache_rows = d->cache.pages * d->cache.kv_heads * d->cache.page_size;
@@ -174,7 +178,7 @@ int launch_attention_tc(txb::KvAttnParams p, const tx_kv_attention_desc *d)
     const int64_t items = d->batch * d->cache.kv_heads * p.row_parts;
     int sms = 0;
     if (int rc = txb::api::sm_count(&sms)) return rc;
-    const int splits = splits_of(d, items, sms, Cfg::MAX_SPLITS, Cfg::BN);
+    const int splits = splits_of(keys_seen(d), items, sms, Cfg::MAX_SPLITS, Cfg::BN);
     if (int rc = allow_launch<txb::kv_attention_tc_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
     return launch_cluster(txb::kv_attention_tc_kernel<Cfg>, items * splits, splits, Cfg::THREADS, Cfg::SMEM, d->stream, p);
 }
@@ -205,6 +209,47 @@ int launch_attention(const txb::KvAttnParams &p, const tx_kv_attention_desc *d)
 }
 
 }  // namespace
+
+namespace txb {
+namespace api {
+
+bool window_step_fits(const tx_sdpa_desc *d)
+{
+    if (d->dtype != TX_DTYPE_F16 || d->lse || (d->d_k != 64 && d->d_k != 128) || !aligned(d->out, 16)) return false;
+    return d->q_heads / d->kv_heads * d->seq_q <= 16 && d->batch * d->kv_heads * d->seq_k * d->d_k / 64 <= 0x7fffffffLL;
+}
+
+int window_step(const tx_sdpa_desc *d, const KvLens &lens, int window, int sinks, int align_end, int *status)
+{
+    KvPlainParams p = {};
+    p.lens = lens;
+    p.Sk = (int)d->seq_k; p.align_end = align_end;
+    p.pages.Hkv = (int)d->kv_heads;
+    p.q = d->q; p.out = d->out; p.status = status;
+    p.tokens = (int)d->seq_q; p.group = (int)(d->q_heads / d->kv_heads);
+    p.window = window; p.sinks = sinks;
+    p.out_f16 = (d->flags & TX_SDPA_OUT_F16) ? 1 : 0;
+    p.scale_log2 = (1.0f / std::sqrt((float)d->d_k)) * 1.4426950408889634f;
+    auto launch = [&](auto cfg) -> int {
+        using Cfg = decltype(cfg);
+        p.row_parts = (p.group * p.tokens + Cfg::MR - 1) / Cfg::MR;
+        const int64_t heads = d->batch * d->kv_heads, items = heads * p.row_parts;
+        int sms = 0;
+        if (int rc = sm_count(&sms)) return rc;
+        const int splits = splits_of(std::min<int64_t>(d->seq_k, (int64_t)window + sinks + d->seq_q), items, (int64_t)Cfg::CTAS_PER_SM * sms,
+                                     Cfg::MAX_SPLITS, Cfg::KT);
+        if (int rc = allow_launch<kv_attention_kernel<Cfg>>((int)Cfg::SMEM)) return rc;
+        CUtensorMap tk, tv;
+        if (int rc = map_of_codes(&tk, d->k, heads * d->seq_k, 2 * d->d_k)) return rc;
+        if (int rc = map_of_codes(&tv, d->v, heads * d->seq_k, 2 * d->d_k)) return rc;
+        return launch_cluster(kv_attention_kernel<Cfg>, items * splits, splits, Cfg::THREADS, Cfg::SMEM, d->stream, tk, tv, p);
+    };
+    if (d->d_k == 64) return launch(KvAttnCfg<__half, KV_PLAIN, 64, 1, 4, 32, 2, 3>());
+    return launch(KvAttnCfg<__half, KV_PLAIN, 128, 1, 4, 16, 2, 3>());
+}
+
+}  // namespace api
+}  // namespace txb
 
 extern "C" {
 

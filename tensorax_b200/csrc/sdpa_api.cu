@@ -1086,6 +1086,8 @@ int window_forward(const tx_sdpa_desc *d, const tx_window_desc *w)
         }
         int *status = nullptr;
         if (int rc = status_word(&status)) return rc;
+        if (route == Route::Decode && txb::api::window_step_fits(e))
+            return txb::api::window_step(e, lens_of(e->kv_lens, e->flags, e->batch), rule.window, rule.sinks, rule.align_end, status);
         if (route == Route::Decode)
             return e->dtype == TX_DTYPE_F16 ? launch_decode<__half, true>(e, st, status, &rule) : launch_decode<float, true>(e, st, status, &rule);
         return route == Route::TensorCores ? launch_tc_window(e, st, status, &rule) : launch_x3(e, st, status, nullptr, &rule);
