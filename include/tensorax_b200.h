@@ -313,7 +313,8 @@ TX_API int tx_sdpa_backward(const tx_sdpa_bwd_desc *desc);
  *      The forward descriptor is that of tx_sdpa_forward with `causal` nonzero and without a dense mask; flags
  *      TX_SDPA_OUT_F16, TX_SDPA_KV_LENS_HOST, TX_SDPA_FORCE_SIMT.  All of its types and head dims, `lse` included.
  *      A row that sees no key is NaN; rows from kv_lens[b] on of K and V may hold anything.  A value that is not finite at a
- *      key that one row of a 128-row tile sees may show in the tile's other rows.
+ *      valid key within 128 keys of one that some row of a 128-row tile sees may show in all rows of the tile (decoding steps of up
+ *      to 16 rows a K/V head: at a key that one of them sees).
  *      Backward: as tx_sdpa_backward (fp16, d in {64, 128, 256}); a row that sees no key has gradient zero and adds nothing to
  *      those of K and V.  TX_BWD_GRADS_F16: dq, dk, dv are fp16. */
 enum { TX_BWD_GRADS_F16 = 64 };
@@ -386,7 +387,7 @@ TX_API int tx_kv_cache_read(const tx_kv_read_desc *desc);
  * into which they have been written.  Sequence b has kv_lens[b] keys of which the last n = q_lens[b] are this call's nodes;
  * ctx = kv_lens[b] - n.  Node t sees key j < ctx (with a window: where j > ctx + depth(t) - window or j < sinks; depth(t) is
  * the number of nodes it sees beside itself) and node u iff bit u of tree[b][t] is set (without `tree`: iff u <= t).  A row that
- * sees nothing is NaN.  Rows of nodes t >= n are left as they were.  fp16 queries: fp16 products, fp32 sums; fp32 queries:
+ * sees nothing is NaN, as are the nodes t >= kv_lens[b] of a sequence shorter than n.  Rows of nodes t >= n are left as they were.  fp16 queries: fp16 products, fp32 sums; fp32 queries:
  * fp32-grade products of the codes' values. */
 typedef struct tx_kv_attention_desc {
     tx_kv_cache cache;

@@ -46,7 +46,7 @@ constexpr int KV_PLAIN = 2;
 struct KvAttnParams {
     KvPages pages;
     const void *q;             // [batch, Hq, tokens, D]
-    void *out;                 // the same, fp32 or fp16 (out_f16); rows of nodes that a sequence does not have stay as they were
+    void *out;                 // the same, fp32 or fp16 (out_f16); rows from q_lens on stay as they were
     const int32_t *kv_lens;    // [batch]: keys of each sequence, this call's nodes among them
     const int32_t *q_lens;     // optional [batch]: nodes of each sequence (none: all)
     const uint64_t *tree;      // optional [batch, tokens]: what a node sees of the nodes (none: node t sees 0 .. t)
@@ -147,6 +147,9 @@ __device__ __forceinline__ int kv_length(const KvAttnParams &p, int b, bool &bey
     return max(0, min(len, p.most_keys));
 }
 
+// Nodes whose rows are written; those that the sequence has no key for get NaN.
+__device__ __forceinline__ int kv_nodes_asked(const KvAttnParams &p, int b) { return p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens; }
+
 // Weights are kept at 2^kKvShift times what they are: the row's largest then leaves fp16 smaller ones room below (2^-30 of
 // it) and room above for a maximum that has grown by less than 2^kKvLazy since the last rescale.
 constexpr float kKvShift = 6.f, kKvLazy = 8.f;
@@ -185,7 +188,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     const int kvh = item / p.row_parts, row0 = (item % p.row_parts) * MR;    // b * Hkv + h, first row of this part
     const int b = kvh / p.pages.Hkv, h = kvh - b * p.pages.Hkv;
     const int rows = p.group * p.tokens;
-    int len, nodes, ctx;                                          // keys of the sequence, rows of a head, position of the first
+    int len, nodes, ctx;                                          // keys of the sequence, nodes among them, position of the first
     if constexpr (PLAIN) {
         len = p.lens.limit(b, p.Sk);
         nodes = p.tokens;
@@ -195,7 +198,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         bool beyond;
         len = kv_length(p, b, beyond);
         if (beyond && tid == 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
-        nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
+        nodes = min(kv_nodes_asked(p, b), len);
         ctx = len - nodes;
     }
     // Visible keys as one range of numbers: the sinks in front of the window, then the keys from the window of the shallowest
@@ -627,10 +630,11 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     __syncthreads();
     // Warps of the CTA: number `i` of MR x D / 4 float4s over them, into the first one's place
     constexpr int QUADS = D / 4;
+    const int asked = PLAIN ? p.tokens : kv_nodes_asked(p, b);
     auto write = [&](int r, int quad, float4 v, float sum) {
-        const int row = row0 + r;
-        if (row >= rows || row % p.tokens >= nodes) return;
-        const float f = *bad || *abort_flag ? __int_as_float(0x7fc00000) : 1.f / sum;               // no visible key: 0 * inf = NaN
+        const int row = row0 + r, node = row % p.tokens;
+        if (row >= rows || node >= asked) return;
+        const float f = *bad || *abort_flag || node >= nodes ? __int_as_float(0x7fc00000) : 1.f / sum;               // no visible key: 0 * inf = NaN
         v.x *= f; v.y *= f; v.z *= f; v.w *= f;
         const int64_t to = ((int64_t)kvh * rows + row) * D + quad * 4;
         if (p.out_f16)

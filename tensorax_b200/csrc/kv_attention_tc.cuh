@@ -129,7 +129,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
     const int rows = p.group * p.tokens;
     bool beyond = false;
     const int len = kv_length(p, b, beyond);
-    const int nodes = min(p.q_lens ? min(max(p.q_lens[b], 0), p.tokens) : p.tokens, len);
+    const int nodes = min(kv_nodes_asked(p, b), len);
     const int ctx = len - nodes;
     int first = 0, s_end = 0;
     if (p.window > 0) {
@@ -539,6 +539,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
         constexpr int U = 4;
+        const int asked = kv_nodes_asked(p, b);
         for (int first_r = (warp - 8) * RPW; first_r < mine; first_r += 8 * RPW * U) {
             float4 acc[U];
 #pragma unroll
@@ -559,7 +560,8 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int rl = first_r + u * 8 * RPW + lane / QUADS, row_o = row0 + r_first + rl;
-                if (rl >= mine || row_o >= rows || row_o % p.tokens >= nodes) continue;
+                if (rl >= mine || row_o >= rows || row_o % p.tokens >= asked) continue;
+                if (row_o % p.tokens >= nodes) acc[u].x = acc[u].y = acc[u].z = acc[u].w = __int_as_float(0x7fc00000);
                 const int64_t to = ((int64_t)kvh * rows + row_o) * D + (lane % QUADS) * 4;
                 if (p.out_f16)
                     *reinterpret_cast<uint2 *>(static_cast<__half *>(p.out) + to) = make_uint2(ptx::pack_half2(acc[u].x, acc[u].y), ptx::pack_half2(acc[u].z, acc[u].w));

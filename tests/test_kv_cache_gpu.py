@@ -354,6 +354,17 @@ def test_rows_of_nodes_that_do_not_exist_stay(lib=None):
     assert (got[0, :, 4:] == -3).all() and (got[1] == -3).all() and (got[0, :, :4] != -3).all()
 
 
+@pytest.mark.parametrize("heads", [2, 60])
+def test_sequences_of_fewer_keys_than_nodes(heads):
+    """An idle place of a batch (no key), and a sequence that is shorter than the call: no key, no result."""
+    cache, table, kv = filled(17, 3, 1, 40, 64, 16, "int8")
+    q = seeded(4, 3, heads, 3, 64).astype(np.float16)
+    for dtype in (np.float16, np.float32) if heads == 2 else (np.float16,):
+        got = cache.attend(tensor(q.astype(dtype)), table, [0, 2, 40]).numpy()
+        assert np.isnan(got[0]).all() and np.isnan(got[1, :, 2]).all()
+        assert np.isfinite(got[1, :, :2]).all() and np.isfinite(got[2]).all()
+
+
 def test_the_same_bits_every_time():
     cache, table, _ = filled(15, 2, 2, 3000, 128, 64, "e4m3")
     q = tensor(seeded(4, 2, 8, 6, 128).astype(np.float16))

@@ -111,6 +111,22 @@ def test_decoding_step(case, d, dtype):
     check(run(q, k, v, window, sinks, lens, "end"), q, k, v, full, window, sinks, "end", dtype == np.float16 and Sk < 128)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("align", ["start", "end"])
+def test_few_rows_with_and_without_the_row_statistic(d, align):
+    """The two kernels for few fp16 rows: the one that leaves the statistic for the backward, and the one that does not."""
+    B, Hq, Hkv, Sq, Sk, window, sinks, lens = 2, 6, 2, 5, 300, 40, 3, [300, 123]
+    q, k, v = (seeded(i, B, h, s, d).astype(np.float16) for i, (h, s) in enumerate(((Hq, Sq), (Hkv, Sk), (Hkv, Sk))))
+    g = seeded(9, B, Hq, Sq, d)
+    check(run(q, k, v, window, sinks, lens, align), q, k, v, lens, window, sinks, align, False)
+    out, got = gradients(q, k, v, g, window, sinks, lens, align)
+    check(out, q, k, v, lens, window, sinks, align, False)
+    for name, a, b in zip("qkv", got, window_oracle.backward(q, k, v, g, lens, window, sinks, align)):
+        assert np.linalg.norm(a - b) <= 2.0 ** -8 * np.linalg.norm(b), name
+    half, _ = gradients(q, k, v, g, window, sinks, lens, align, "float16", "float16")
+    assert np.abs(half.astype(np.float32) - out).max() <= 2.0 ** -11 * np.abs(out).max()
+
+
 def test_what_lies_behind_the_last_key_may_be_anything():
     for d, dtype in ((64, np.float16), (128, np.float16), (256, np.float16), (64, np.float32), (160, np.float32)):
         q, k, v = (seeded(i, 2, 2, 400, d).astype(dtype) for i in range(3))
