@@ -1932,8 +1932,12 @@ static int backward_launch(const tx_sdpa_bwd_desc *d, const txb::WindowRule *win
     int *prepared = reinterpret_cast<int *>(ws + h_bytes + delta_bytes);
     auto prep = [&](auto out, auto dim) {
         constexpr int D = decltype(dim)::value, rows_per_cta = 8 * 2 * (D == 64 ? 2 : 1);
-        txb::sdpa_bwd_prep_kernel<std::remove_const_t<std::remove_pointer_t<decltype(out)>>, D>
-            <<<(unsigned)((rows + rows_per_cta - 1) / rows_per_cta), 256, 0, st>>>(d->dout, out, dout_h, delta, rows, prepared);
+        using OT = std::remove_const_t<std::remove_pointer_t<decltype(out)>>;
+        const unsigned ctas = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
+        if (win) {
+            const txb::PrepWindow pw = {lens_of(d->kv_lens, d->flags, d->batch), *win, (int)d->q_heads, (int)d->seq_q, (int)d->seq_k, d->lse};
+            txb::sdpa_bwd_prep_kernel<OT, D, true><<<ctas, 256, 0, st>>>(d->dout, out, dout_h, delta, rows, prepared, pw);
+        } else txb::sdpa_bwd_prep_kernel<OT, D, false><<<ctas, 256, 0, st>>>(d->dout, out, dout_h, delta, rows, prepared, 0);
     };
     auto prep_of = [&](auto out) {
         if (d->d == 64) prep(out, std::integral_constant<int, 64>{});

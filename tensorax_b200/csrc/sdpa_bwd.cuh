@@ -169,10 +169,25 @@ __device__ __forceinline__ void store_grad_half(const uint8_t *tile, __half *dst
 // dO fp32 -> fp16 (MMA operand) and delta = rowsum(dO o O).  Bound: HBM (10 d + 4 or 8 d + 4 bytes a row).  Sixteen lanes a row
 // at d = 64, 32 otherwise, four values a lane and step; a warp requests two steps of rows at a time.  One row a warp and
 // eight bytes a lane took 30.3 us at B4 H16 S2048 d128, this 23.4 (6.9 TB/s; dO and O partly in L2).
-template <typename OT, int D>
+// With a window a row that sees no key gets dO and delta zero, whatever the caller's gradient of its NaN is: in the products that
+// add up dK and dV its weight of zero would not keep a NaN out.
+struct PrepWindow {
+    KvLens kv_lens;
+    WindowRule rule;
+    int Hq, Sq, Sk;
+    const float *lse;
+    __device__ __forceinline__ bool sees_none(int64_t row, float row_lse) const
+    {
+        if (row_lse > -1.0e29f) return false;                     // most rows: no division
+        const int64_t head = row / Sq;
+        const int limit = kv_lens.limit((int)(head / Hq), Sk), pos = rule.offset(limit, Sq) + (int)(row - head * Sq);
+        return limit <= 0 || pos < 0 || (rule.sinks <= 0 && pos - rule.window + 1 >= limit);
+    }
+};
+template <typename OT, int D, bool WINDOW>
 __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restrict__ dout, const OT *__restrict__ out,
                                                             __half *__restrict__ dout_h, float *__restrict__ delta, int64_t rows,
-                                                            int *prepared)
+                                                            int *prepared, const __grid_constant__ std::conditional_t<WINDOW, PrepWindow, int> window)
 {
     ptx::grid_trigger();
     if (blockIdx.x == 0 && threadIdx.x == 0) *prepared = 0;
@@ -180,6 +195,7 @@ __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restr
     const int lane = threadIdx.x & 31, gl = lane % LPR;
     const int64_t row0 = ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * (RPW * STEPS) + lane / LPR;
     float4 g[STEPS][PIECES], o[STEPS][PIECES];
+    float row_lse[STEPS];
 #pragma unroll
     for (int t = 0; t < STEPS; ++t)
 #pragma unroll
@@ -187,6 +203,8 @@ __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restr
             const int64_t row = row0 + t * RPW;
             g[t][c] = o[t][c] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (row >= rows) continue;
+            if constexpr (WINDOW)
+                if (c == 0) row_lse[t] = __ldg(window.lse + row);
             const int64_t at = row * D + (c * LPR + gl) * 4;
             g[t][c] = *reinterpret_cast<const float4 *>(dout + at);
             if constexpr (sizeof(OT) == 2) {
@@ -201,6 +219,10 @@ __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restr
     for (int t = 0; t < STEPS; ++t) {
         const int64_t row = row0 + t * RPW;
         float acc = 0.f;
+        if constexpr (WINDOW)
+            if (row < rows && window.sees_none(row, row_lse[t]))
+#pragma unroll
+                for (int c = 0; c < PIECES; ++c) g[t][c] = o[t][c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) {
             const float4 a = g[t][c], b = o[t][c];
@@ -870,8 +892,8 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             // that none of them is left behind at it.
             const int qr0 = (i_start + i_n) * BQ;
             float *st_lse = stat + (t & 1) * 2 * BQ, *st_delta = st_lse + BQ;
-            // (a row that sees no key, window: its sum is nothing and its maximum the stand-in, its delta 0/0)
-            if (Cfg::WINDOW && (st < BQ ? next_stat < -1.0e29f : next_stat != next_stat)) next_stat = st < BQ ? INFINITY : 0.f;
+            // (a row that sees no key, window: its sum is nothing and its maximum the stand-in, or NaN and masked)
+            if (Cfg::WINDOW && st < BQ && next_stat < -1.0e29f) next_stat = INFINITY;
             if (st < 2 * BQ) st_lse[st] = stat_mul * next_stat;
             if constexpr (Cfg::WGS == 1) asm volatile("bar.sync 1, 128;" ::: "memory");
             else asm volatile("bar.sync 1, 256;" ::: "memory");

@@ -233,6 +233,22 @@ def test_what_lies_behind_the_last_key_has_no_part_in_gradients():
         assert all(np.array_equal(a, b) for a, b in zip(got, clean))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens, align, sinks", [([200, 700], "start", 0), ([300, 0], "end", 2), ([690, 128], "end", 20)])
+def test_gradients_of_rows_that_see_nothing_are_not_read(d, lens, align, sinks):
+    """A loss over all rows hands the NaN of rows without keys back as their gradient: it goes nowhere."""
+    B, H, S, window = 2, 2, 700, 64
+    q, k, v = (seeded(i, B, H, S, d).astype(np.float16) for i in range(3))
+    g = seeded(5, B, H, S, d)
+    _, clean = gradients(q, k, v, g, window, sinks, lens, align)
+    dead = np.stack([~window_oracle.seen(S, S, n, window, sinks, align).any(1) for n in lens])
+    assert dead.any()
+    for b in range(B):
+        g[b][:, dead[b]] = np.nan
+    _, got = gradients(q, k, v, g, window, sinks, lens, align)
+    assert all(np.isfinite(a).all() and np.array_equal(a, b) for a, b in zip(got, clean))
+
+
 def test_gradients_against_differences():
     """Central differences of the kernel's own forward pass, along random directions.  fp32 results of fp16 products: a loss
     of n terms is off by about 2^-11 sqrt(n) |g||o| / sqrt(n); the step is large enough for that to be a few per cent."""
