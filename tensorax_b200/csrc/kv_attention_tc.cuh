@@ -3,7 +3,7 @@
 //
 // Bound: the tensor pipe and the softmax's exponentials, as in sdpa_tc_pair_kernel, whose softmax, issue order and tensor-memory
 // layout (P over S) this kernel has.  mma.sync, which the other kernel uses, does a third of tcgen05's work at best (549 TFLOP/s
-// measured); at 256 rows a head it took 341 us where this kernel takes 109 us (B8 Hkv8, 8192 keys in the window, d 128: 634 TFLOP/s).
+// measured); at 256 rows a head it took 341 us where this kernel takes 101 us (B8 Hkv8, 8192 keys in the window, d 128: 683 TFLOP/s).
 //
 // One CTA: two 128-row query tiles of one (batch, K/V head) and a share of the keys in tiles of 128; CTAs of a cluster share the
 // keys and add their results in rank order.
@@ -314,15 +314,12 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         for (int n = 0; n < MINE; ++n) request(0, w + W * n);
         for (int j = 0; j < n_tiles && ok; ++j) {
             float kf[4], vf[4];
-            uint32_t kh[4], vh[4], ktop = 0, vtop = 0;
-            bool fine[4];
+            uint32_t factor[MINE], ktop = 0, vtop = 0;            // the lane's of the units, as key lane of the 32 that hold the unit
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 kf[e] = kc[e]; vf[e] = vc[e];
-                fine[e] = kf[e] < INFINITY && vf[e] < INFINITY;   // neither NaN nor infinite
-                if (fine[e]) { ktop = max(ktop, __float_as_uint(kf[e])); vtop = max(vtop, __float_as_uint(vf[e])); }
+                if (kf[e] < INFINITY && vf[e] < INFINITY) { ktop = max(ktop, __float_as_uint(kf[e])); vtop = max(vtop, __float_as_uint(vf[e])); }
             }
-            ask(j + 1);
             const uint32_t kref = kv_pow2_above(__reduce_max_sync(0xffffffffu, ktop));
             vref = max(vref, kv_pow2_above(__reduce_max_sync(0xffffffffu, vtop)));
             if (w == 0 && lane == 0) {
@@ -332,12 +329,16 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
             }
             const float k_inv = __uint_as_float((254u << 23) - kref), v_inv = __uint_as_float((254u << 23) - vref);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                kh[e] = kv_factor<FMT>(fine[e] ? kf[e] * k_inv : __int_as_float(0x7fc00000));
-                vh[e] = kv_factor<FMT>(fine[e] ? vf[e] * v_inv : 0.f);
+            for (int n = 0; n < MINE; ++n) {
+                const int u = w + W * n, g = u % Cfg::UNITS, e = g >> 1;
+                const bool of_k = u < Cfg::UNITS;
+                const float kq = e < 2 ? (e == 0 ? kf[0] : kf[1]) : (e == 2 ? kf[2] : kf[3]), vq = e < 2 ? (e == 0 ? vf[0] : vf[1]) : (e == 2 ? vf[2] : vf[3]);
+                const bool ok_key = kq < INFINITY && vq < INFINITY;
+                factor[n] = kv_factor<FMT>(of_k ? (ok_key ? kq * k_inv : __int_as_float(0x7fc00000)) : (ok_key ? vq * v_inv : 0.f));
             }
+            ask(j + 1);
             bool k_done = false;
-#pragma unroll 1
+#pragma unroll
             for (int n = 0; n < MINE && ok; ++n) {
                 const int u = w + W * n, g = u % Cfg::UNITS;
                 const bool of_k = u < Cfg::UNITS;
@@ -355,14 +356,12 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
                 if (j > 1) ok = ptx::mbar_wait((of_k ? k_free : v_free) + 8 * (j & 1), (uint32_t)((j >> 1) - 1) & 1u, abort_flag);
                 if (ok && u < 2 * Cfg::UNITS) {
                     uint8_t *dst = smem + (of_k ? Cfg::OFF_K : Cfg::OFF_V) + (j & 1) * Cfg::KV_TILE + g * 2048;
-                    const uint32_t factor = of_k ? (g < 4 ? (g < 2 ? kh[0] : kh[1]) : (g < 6 ? kh[2] : kh[3]))
-                                                 : (g < 4 ? (g < 2 ? vh[0] : vh[1]) : (g < 6 ? vh[2] : vh[3]));
 #pragma unroll
                     for (int i = 0; i < PASSES; ++i) {
                         // four rows further the swizzle's third bit changes, eight rows further nothing does
                         const uint32_t at = (at0 ^ (STEP == 4 && (i & 1) ? 64u : 0u)) + i * STEP * 128;
                         uint4 out[2];
-                        kv_scaled16<FMT>(x[i], __shfl_sync(0xffffffffu, factor, (g & 1) * 16 + r0 + i * STEP), out);
+                        kv_scaled16<FMT>(x[i], __shfl_sync(0xffffffffu, factor[n], (g & 1) * 16 + r0 + i * STEP), out);
                         *reinterpret_cast<uint4 *>(dst + at) = out[0];
                         *reinterpret_cast<uint4 *>(dst + (at ^ 16u)) = out[1];
                     }
