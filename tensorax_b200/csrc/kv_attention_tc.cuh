@@ -3,7 +3,7 @@
 //
 // Bound: the tensor pipe and the softmax's exponentials, as in sdpa_tc_pair_kernel, whose softmax, issue order and tensor-memory
 // layout (P over S) this kernel has.  mma.sync, which the other kernel uses, does a third of tcgen05's work at best (549 TFLOP/s
-// measured); at 256 rows a head it took 341 us where this kernel takes 101 us (B8 Hkv8, 8192 keys in the window, d 128: 683 TFLOP/s).
+// measured); at 256 rows a head it took 341 us where this kernel takes 95 us (B8 Hkv8, 8192 keys in the window, d 128: 724 TFLOP/s).
 //
 // One CTA: two 128-row query tiles of one (batch, K/V head) and a share of the keys in tiles of 128; CTAs of a cluster share the
 // keys and add their results in rank order.
@@ -267,22 +267,21 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
                 page = (pos >> p.pages.page_shift) < p.pages.table_len
                            ? __ldg(p.pages.table + (int64_t)b * p.pages.table_len + (pos >> p.pages.page_shift)) : -1;
         };
-        // first row of the tile's g-th sixteen, or -1: from the pages looked up last
-        auto first_row = [&](int j) -> int64_t {
+        // first row of the tile's g-th sixteen (rows of a cache are 31-bit numbers), or -1: from the pages looked up last
+        auto first_row = [&](int j) -> int {
             const int c = c_from + j * BN + lane * 16, pos = c < s_end ? c : c + skip;
             if (page == -2) return -1;
             if (page < 0 || page >= p.pages.pages) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); return -1; }
-            return ((((int64_t)page * p.pages.Hkv + h) << p.pages.page_shift)) + (pos & ((1 << p.pages.page_shift) - 1));
+            return ((page * p.pages.Hkv + h) << p.pages.page_shift) + (pos & ((1 << p.pages.page_shift) - 1));
         };
         float kc[4], vc[4];                                       // scales of keys lane, lane + 32, ... of a tile
-        int64_t mine = -1;                                        // lane g: first row of the g-th sixteen of the tile asked for
-        auto ask = [&](int j) {                                   // scales of tile j, pages of the one behind it
-            mine = first_row(j);
-            look_up(j + 1);
+        int mine = -1;                                        // lane g: first row of the g-th sixteen of the tile asked for
+        auto turn = [&](int j) { mine = first_row(j); look_up(j + 1); };      // rows of tile j, pages of the one behind it
+        auto ask = [&](int j) {                                   // scales of that tile
             const int left = c_to - (c_from + j * BN);            // keys that the tile has
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int64_t row = __shfl_sync(0xffffffffu, mine, 2 * e + (lane >> 4));
+                const int row = __shfl_sync(0xffffffffu, mine, 2 * e + (lane >> 4));
                 const bool there = row >= 0 && e * 32 + lane < left;
                 kc[e] = there ? __ldg(p.pages.ks + row + (lane & 15)) : 0.f;
                 vc[e] = there ? __ldg(p.pages.vs + row + (lane & 15)) : 0.f;
@@ -290,10 +289,10 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         };
         auto request = [&](int j, int u) {                        // codes of unit u of tile j, the tile asked for last
             const int g = u % Cfg::UNITS, left = c_to - (c_from + j * BN) - g * 16;
-            const int64_t row = __shfl_sync(0xffffffffu, mine, g);
+            const int row = __shfl_sync(0xffffffffu, mine, g);
             if (u < 2 * Cfg::UNITS && j < n_tiles) {
                 const uint32_t dst = ptx::smem_u32(codes + u * Cfg::UNIT);
-                const uint8_t *from = (u < Cfg::UNITS ? p.pages.k : p.pages.v) + (row >= 0 ? (row + r0) * D + chunk * 16 : 0);
+                const uint8_t *from = (u < Cfg::UNITS ? p.pages.k : p.pages.v) + (row >= 0 ? (int64_t)(row + r0) * D + chunk * 16 : 0);
                 if (row >= 0 && left >= 16) {
 #pragma unroll
                     for (int i = 0; i < PASSES; ++i) ptx::cp_async16(dst + i * 512, from + i * STEP * D);
@@ -310,6 +309,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         bool ok = true;
         uint32_t vref = 1u << 23;
         look_up(0);
+        turn(0);
         ask(0);
         for (int n = 0; n < MINE; ++n) request(0, w + W * n);
         for (int j = 0; j < n_tiles && ok; ++j) {
@@ -336,7 +336,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
                 const bool ok_key = kq < INFINITY && vq < INFINITY;
                 factor[n] = kv_factor<FMT>(of_k ? (ok_key ? kq * k_inv : __int_as_float(0x7fc00000)) : (ok_key ? vq * v_inv : 0.f));
             }
-            ask(j + 1);
+            turn(j + 1);
             bool k_done = false;
 #pragma unroll
             for (int n = 0; n < MINE && ok; ++n) {
@@ -353,6 +353,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
 #pragma unroll
                 for (int i = 0; i < PASSES; ++i) x[i] = *reinterpret_cast<const uint4 *>(codes + min(u, 15) * Cfg::UNIT + i * 512);
                 request(j + 1, u);
+                if (n == 0) ask(j + 1);                           // (in front of the units: 103 us for 98)
                 if (j > 1) ok = ptx::mbar_wait((of_k ? k_free : v_free) + 8 * (j & 1), (uint32_t)((j >> 1) - 1) & 1u, abort_flag);
                 if (ok && u < 2 * Cfg::UNITS) {
                     uint8_t *dst = smem + (of_k ? Cfg::OFF_K : Cfg::OFF_V) + (j & 1) * Cfg::KV_TILE + g * 2048;
