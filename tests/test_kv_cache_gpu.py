@@ -482,6 +482,61 @@ def test_calls_in_two_graphs_and_on_two_streams():
         assert all(torch.equal(job[3], w) for job, w in zip(jobs, want))
 
 
+@pytest.mark.parametrize("T", [1, 24])
+def test_calls_that_follow_each_other_without_a_wait(T):
+    """Queries, keys, lengths and pages are written on the stream right in front of the calls that read them, and overwritten
+    right behind: the same bits as with a wait after every step."""
+    torch = pytest.importorskip("torch")
+    lib, stream = _lib.load(), torch.cuda.Stream()
+    st = ctypes.c_void_p(stream.cuda_stream)
+    B, Hq, Hkv, d, page, table_len, steps = 2, 8, 2, 128, 16, 40, 12
+    generator = torch.Generator(device="cuda").manual_seed(1)
+    new = [torch.randn(steps, B, Hkv, T, d, generator=generator, device="cuda").half() for _ in range(2)]
+    qs = torch.randn(steps, B, Hq, T, d, generator=generator, device="cuda").half()
+    plain = [torch.randn(B, Hkv, 640, d, generator=generator, device="cuda").half() for _ in range(2)]
+    tables = torch.stack([torch.randperm(B * table_len).view(B, table_len) for _ in range(steps)]).int().cuda()
+
+    def run(wait):
+        codes, scales = [torch.zeros(B * table_len, Hkv, page, d, dtype=torch.uint8, device="cuda") for _ in range(2)], \
+                        [torch.zeros(B * table_len, Hkv, page, device="cuda") for _ in range(2)]
+        k, v, q = torch.zeros_like(new[0][0]), torch.zeros_like(new[1][0]), torch.zeros_like(qs[0])
+        table, start, lens = torch.zeros_like(tables[0]), torch.zeros(B, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+        out, step_out = torch.zeros(B, Hq, T, d, device="cuda"), torch.zeros(B, Hq, 1, d, device="cuda")
+        q1 = torch.zeros(B, Hq, 1, d, dtype=torch.float16, device="cuda")
+        cache = _lib.KvCache(k=codes[0].data_ptr(), v=codes[1].data_ptr(), k_scale=scales[0].data_ptr(), v_scale=scales[1].data_ptr(),
+                             pages=B * table_len, kv_heads=Hkv, page_size=page, d=d, format=_lib.TX_KV_E4M3)
+        write = _lib.KvWriteDesc(cache=cache, k=k.data_ptr(), v=v.data_ptr(), page_table=table.data_ptr(), start=start.data_ptr(),
+                                 batch=B, tokens=T, table_len=table_len, dtype=_lib.TX_DTYPE_F16, stream=st)
+        attend = _lib.KvAttentionDesc(cache=cache, q=q.data_ptr(), out=out.data_ptr(), page_table=table.data_ptr(), kv_lens=lens.data_ptr(),
+                                      batch=B, q_heads=Hq, tokens=T, table_len=table_len, dtype=_lib.TX_DTYPE_F16, stream=st)
+        window = _lib.SdpaDesc(q=q1.data_ptr(), k=plain[0].data_ptr(), v=plain[1].data_ptr(), kv_lens=lens.data_ptr(), out=step_out.data_ptr(),
+                               batch=B, q_heads=Hq, kv_heads=Hkv, seq_q=1, seq_k=640, d_k=d, d_v=d, dtype=_lib.TX_DTYPE_F16, causal=1, stream=st)
+        rule, got = _lib.WindowDesc(window=50, sinks=2, align_end=1), []
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            for i in range(steps):
+                for to, x in ((k, new[0][i]), (v, new[1][i]), (q, qs[i]), (table, tables[i]), (q1, qs[i][:, :, :1])):
+                    to.copy_(x)
+                start.fill_(16 * i)
+                _lib.check(lib.tx_kv_cache_write(ctypes.byref(write)))
+                lens.fill_(16 * i + T)
+                _lib.check(lib.tx_kv_cache_attention(ctypes.byref(attend)))
+                _lib.check(lib.tx_sdpa_window_forward(ctypes.byref(window), ctypes.byref(rule)))
+                for x in (q, q1, k, v):
+                    x.fill_(float("nan"))
+                got += [out.clone(), step_out.clone()]
+                if wait:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        _lib.check(lib.tx_sdpa_finish(st))
+        return got
+
+    want = run(True)
+    assert all(torch.isfinite(x).all() for x in want[1::2])
+    for _ in range(3):
+        assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(run(False), want))
+
+
 def test_functional_refusals():
     cache = QuantizedKVCache(4, 2, 64, 16)
     x = tensor(seeded(1, 1, 2, 3, 64))

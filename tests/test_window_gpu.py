@@ -319,6 +319,34 @@ def test_forward_and_backward_in_a_graph_beside_an_eager_step(d):
         assert all(torch.equal(a, b) for a, b in zip((out, *grads), want))
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_decoding_step_in_a_graph(d):
+    """Recorded once, replayed as the sequences grow: lengths and queries are read when it runs."""
+    torch = pytest.importorskip("torch")
+    lib, stream = _lib.load(), torch.cuda.Stream()
+    B, Hq, Hkv, S = 3, 8, 2, 500
+    q = torch.empty(B, Hq, 1, d, device="cuda", dtype=torch.float16).normal_()
+    k, v = (torch.empty(B, Hkv, S, d, device="cuda", dtype=torch.float16).normal_() for _ in range(2))
+    out, lens = torch.zeros(B, Hq, 1, d, device="cuda"), torch.tensor([100, 1, 499], dtype=torch.int32, device="cuda")
+    desc = _lib.SdpaDesc(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), kv_lens=lens.data_ptr(), out=out.data_ptr(), batch=B, q_heads=Hq,
+                         kv_heads=Hkv, seq_q=1, seq_k=S, d_k=d, d_v=d, dtype=_lib.TX_DTYPE_F16, causal=1, stream=ctypes.c_void_p(stream.cuda_stream))
+    win = _lib.WindowDesc(window=70, sinks=3, align_end=1)
+    torch.cuda.synchronize()
+    _lib.check(lib.tx_sdpa_window_forward(ctypes.byref(desc), ctypes.byref(win)))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="relaxed"):
+        _lib.check(lib.tx_sdpa_window_forward(ctypes.byref(desc), ctypes.byref(win)))
+    for step in range(4):
+        q.normal_()
+        lens.copy_(torch.tensor([100 + 100 * step, 1 + step, 499], dtype=torch.int32))
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out.cpu().numpy(), *(x.cpu().numpy() for x in (q, k, v)), lens.tolist(), 70, 3, "end", False)
+
+
 # ------------------------------------------------------------------ as they are used
 def test_prompt_in_chunks_then_steps():
     """A layer with a window: the whole prompt at once, the same in chunks against what has been kept, single tokens against
