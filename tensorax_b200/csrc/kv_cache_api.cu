@@ -183,16 +183,19 @@ int launch_attention_tc(txb::KvAttnParams p, const tx_kv_attention_desc *d)
     return launch_cluster(txb::kv_attention_tc_kernel<Cfg>, items * splits, splits, Cfg::THREADS, Cfg::SMEM, d->stream, p);
 }
 
-// More query rows per K/V head than this: the tcgen05 kernel, whose CTA takes 256 at once.  B8 Hkv8 d128, 8192 keys: 32 rows a head
-// 57 us here and 96 there, 64 rows 94 and 98, 128 rows 162 and 100; B1, 2000 keys: 64 rows 33 and 29.
-constexpr int kTcRows = 64;
+// More query rows per K/V head than this: the tcgen05 kernel, whose CTA takes 256 at once.  Hkv8, us there and here, e4m3:
+// B8, 8192 keys, d128: 32 rows 81 and 50, 64 rows 82 and 86; d64: 65 and 35, 65 and 63; B1, 2000 keys, d128: 18 and 16, 19 and 26;
+// B16, 1000 keys: 28 and 24, 29 and 31.  int8, whose codes take longer to turn into fp16: 64 rows 105 and 94, 73 and 65, 20 and 26,
+// 35 and 33.  128 rows, e4m3, B8: 83 and 162.
+template <int FMT>
+constexpr int kTcRows = FMT == txb::KV_E4M3 ? 32 : 64;
 
 template <typename T, int FMT, int D>
 int launch_attention(const txb::KvAttnParams &p, const tx_kv_attention_desc *d)
 {
     const int64_t rows = (int64_t)p.group * p.tokens;
     if constexpr (sizeof(T) == 2 && D <= 128)
-        if (rows > kTcRows) return launch_attention_tc<txb::KvTcCfg<FMT, D, D == 64 ? 0x0303 : 0x0003>>(p, d);
+        if (rows > kTcRows<FMT>) return launch_attention_tc<txb::KvTcCfg<FMT, D, D == 64 ? 0x0303 : 0x0003>>(p, d);
     // Rows of a part: eight at a time up to 32 (16 at d = 256), as registers hold them.  Steps of 32 keys where registers allow
     // (B16 Hkv8, 8192 keys, d128: four rows 67.6 us with 32 keys a step and three CTAs an SM, 69.7 with 16 and four; sixteen
     // rows 71.7 and 101; 32 rows a head at 256 in all 352 and 463).
