@@ -483,8 +483,9 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
             ptx::tc_fence_after_sync();
         }
         if (run && nt > 0 && !ok) { *abort_flag = 1; ptx::report(p.status, KV_TC_ERR_SOFTMAX); }
-        // the row's max and sum: a row without a key has neither (the polynomial's 2^(-inf) is not quite 0)
-        if (m_used == -1.0e30f) l = 0.f;
+        // the row's max and sum: a row without a key has neither (the polynomial's 2^(-inf) is not quite 0).  A sum that is NaN stays:
+        // the row sees a key that is not finite, here perhaps that alone.
+        if (m_used == -1.0e30f && l == l) l = 0.f;
         ml[t * BM + r] = make_float2(m_used, l);
         // both tiles' MMAs are done before the operands make room for the result
         asm volatile("bar.sync 1, 256;" ::: "memory");
