@@ -426,12 +426,12 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < BN; i += 8) {
-                mx0 = ptx::max3(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-                mx1 = ptx::max3(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
-                mx2 = ptx::max3(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
-                mx3 = ptx::max3(mx3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
+                mx0 = ptx::max3_nan(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                mx1 = ptx::max3_nan(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+                mx2 = ptx::max3_nan(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
+                mx3 = ptx::max3_nan(mx3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
             }
-            const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+            const float mx = ptx::max3_nan(ptx::max3_nan(mx0, mx1, mx2), mx3, mx3);
             const float m_new = fmaxf(m_used, mx * scale);
             const float m_next = (m_new > m_used + kLazyRescaleLog2) ? m_new : m_used;
             const float alpha = ptx::ex2_approx(m_used - m_next);
@@ -455,6 +455,8 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
                 pk[i / 2 + 1] = ptx::pack_half2(eb.x, eb.y);
             }
             l = l * alpha + ((sum_a.x + sum_a.y) + (sum_b.x + sum_b.y));
+            // a score of NaN or +inf makes the row NaN; the polynomial exponential alone would drop it
+            if (!(mx < INFINITY)) l = __int_as_float(0x7fc00000);
             if (j > 0) {
                 ok = ptx::mbar_wait(pv_done + 8 * t, (uint32_t)(j - 1) & 1u, abort_flag);
                 if (!ok) break;

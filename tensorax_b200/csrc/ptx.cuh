@@ -528,7 +528,7 @@ __device__ __forceinline__ float ex2_poly(float x)
 // 1.5*2^23 trick, degree-3 polynomial for 2^f on f = x - n in [-0.5, 0.5] (max relative error
 // 1.6e-4, a third of the fp16 rounding P gets anyway), n added into the exponent field.
 // Inputs below -126 (masked scores are -inf) are clamped and come out as ~1e-38, which the
-// fp16 conversion turns into 0.
+// fp16 conversion turns into 0.  So does a NaN: a softmax that uses this keeps it by its maximum (max3_nan).
 __device__ __forceinline__ float2 ex2_poly2(float2 x)
 {
     x.x = fmaxf(x.x, -126.0f);
@@ -551,6 +551,13 @@ __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The same, but NaN where one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c)
+{
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)

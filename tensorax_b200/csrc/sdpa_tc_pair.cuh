@@ -454,12 +454,12 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
             for (int i = 0; i < CN; i += 8) {
-                mx0 = ptx::max3(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-                mx1 = ptx::max3(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
-                mx2 = ptx::max3(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
-                mx3 = ptx::max3(mx3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
+                mx0 = ptx::max3_nan(mx0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                mx1 = ptx::max3_nan(mx1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+                mx2 = ptx::max3_nan(mx2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
+                mx3 = ptx::max3_nan(mx3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
             }
-            const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+            const float mx = ptx::max3_nan(ptx::max3_nan(mx0, mx1, mx2), mx3, mx3);
             const float m_new = fmaxf(m_used, mx * scale);
             const float m_next = (m_new > m_used + kLazyRescaleLog2) ? m_new : m_used;
             const float alpha = ptx::ex2_approx(m_used - m_next);   // 1 when the max is kept
@@ -482,6 +482,8 @@ sdpa_tc_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 pk[i / 2 + 1] = ptx::pack_half2(eb.x, eb.y);
             }
             l = l * alpha + ((sum_a.x + sum_a.y) + (sum_b.x + sum_b.y));
+            // a score of NaN or +inf makes the row NaN; the polynomial exponential alone would drop it
+            if (!(mx < INFINITY)) l = __int_as_float(0x7fc00000);
             tick(PSEC_SM_EXP);
             if (j > 0) {
                 // PV of the previous tile must be finished before P is overwritten or O rescaled (with P in

@@ -9,7 +9,7 @@ from tensorax_b200.nn import QuantizedKVCache
 
 pytestmark = pytest.mark.gpu
 
-LEAVES = [3, 7]
+LEAVES = [1, 2, 3, 7, 9]
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
