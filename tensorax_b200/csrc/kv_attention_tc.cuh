@@ -260,17 +260,18 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         uint8_t *codes = smem + Cfg::OFF_CODES + lane * 16;
 
         int page = -1;                                            // lane g: of the g-th sixteen of the tile looked up last
+        // (any number may stand in a page table: whether a lane has a sixteen is not to be told from its page)
+        auto wanted = [&](int j) { return j < n_tiles && lane < Cfg::UNITS && c_from + j * BN + lane * 16 < c_to; };
         auto look_up = [&](int j) {
             const int c = c_from + j * BN + lane * 16, pos = c < s_end ? c : c + skip;
-            page = -2;
-            if (j < n_tiles && lane < Cfg::UNITS && c < c_to)
-                page = (pos >> p.pages.page_shift) < p.pages.table_len
-                           ? __ldg(p.pages.table + (int64_t)b * p.pages.table_len + (pos >> p.pages.page_shift)) : -1;
+            page = -1;
+            if (wanted(j) && (pos >> p.pages.page_shift) < p.pages.table_len)
+                page = __ldg(p.pages.table + (int64_t)b * p.pages.table_len + (pos >> p.pages.page_shift));
         };
         // first row of the tile's g-th sixteen (rows of a cache are 31-bit numbers), or -1: from the pages looked up last
         auto first_row = [&](int j) -> int {
             const int c = c_from + j * BN + lane * 16, pos = c < s_end ? c : c + skip;
-            if (page == -2) return -1;
+            if (!wanted(j)) return -1;
             if (page < 0 || page >= p.pages.pages) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); return -1; }
             return ((page * p.pages.Hkv + h) << p.pages.page_shift) + (pos & ((1 << p.pages.page_shift) - 1));
         };
