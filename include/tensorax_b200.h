@@ -209,7 +209,8 @@ TX_API int tx_sdpa_forward(const tx_sdpa_desc *desc);
  * check of the asynchronous entry points (tx_sdpa_forward, tx_sdpa_backward, tx_linear_f32_cuda): a caller that
  * synchronises some other way does not learn that a kernel gave up (its rows then read NaN).  The status word is one
  * per device and stays set until a tx_sdpa_finish call on that device reports and clears it; launches issued in
- * between return at once and write NaN. */
+ * between return at once and write NaN.  A page or row that does not exist (K/V cache calls) has a word of its own, which the next
+ * tx_sdpa_finish on the device reports and clears too, and which stops nothing: only the sequences concerned are NaN. */
 TX_API int tx_sdpa_finish(void *stream);
 /* 1 if tx_sdpa_forward runs `desc` on a tcgen05 kernel (fp16, or fp32 as hi/lo fp16 pairs), 0 if on CUDA cores: calls
  * with few query rows per K/V head -- decoding steps, up to 16 rows in fp16 and 32 in fp32 -- and small fp32 calls, which the
@@ -339,7 +340,8 @@ TX_API int tx_sdpa_window_backward(const tx_sdpa_bwd_desc *desc, const tx_window
  *      All pointers are device pointers (k, v, q, out, the codes and the scales 16-byte aligned), everything is asynchronous on `stream`
  *      and captures into graphs; no call allocates.  A token without a page (a position beyond the table, an entry outside
  *      [0, pages)) is left out, never followed, and reported: tx_sdpa_finish then returns TX_ERR_KERNEL (stage code 51), and
- *      attention rows of the sequences concerned are NaN. */
+ *      attention rows of the sequences concerned are NaN.  The call's other sequences, and calls behind it, are what they are
+ *      without it. */
 enum { TX_KV_E4M3 = 0, TX_KV_INT8 = 1 };
 typedef struct tx_kv_cache {
     void *k, *v;              /* [pages, kv_heads, page_size, d] codes, a byte each */

@@ -9,13 +9,14 @@
 
 namespace txb {
 
-enum : int { KV_ERR_PAGE = 51 };      // failure word: see kv_cache.cuh
+enum : int { KV_ERR_PAGE = 51 };      // the only code of api::page_word
 
 namespace api {
 
 int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));   // sets tx_last_error(), returns code
 int ensure_device();
-int status_word(int **out);          // the current device's failure word
+int status_word(int **out);          // the current device's failure word: while it is set, kernels that look at it stop
+int page_word(int **out);            // ... and the word for pages and rows that do not exist, which stops nothing
 int sm_count(int *n);
 int current_device(int *dev);
 // `rows` rows of d one-byte codes as 128-byte lines, copied sixteen rows at a time with a 128-byte swizzle

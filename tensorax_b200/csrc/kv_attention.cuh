@@ -50,7 +50,7 @@ struct KvAttnParams {
     const int32_t *kv_lens;    // [batch]: keys of each sequence, this call's nodes among them
     const int32_t *q_lens;     // optional [batch]: nodes of each sequence (none: all)
     const uint64_t *tree;      // optional [batch, tokens]: what a node sees of the nodes (none: node t sees 0 .. t)
-    int *status;
+    int *status, *page_status; // waits that ran out; pages that do not exist (no part of plain keys)
     int most_keys;             // what a page table can hold
     int tokens, group;         // group = Hq / Hkv
     int row_parts;             // CTAs (per split) that share the rows of a head, MR each
@@ -197,7 +197,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
     } else {
         bool beyond;
         len = kv_length(p, b, beyond);
-        if (beyond && tid == 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
+        if (beyond && tid == 0) { *bad = 1; ptx::report(p.page_status, KV_ERR_PAGE); }
         nodes = min(kv_nodes_asked(p, b), len);
         ctx = len - nodes;
     }
@@ -251,7 +251,7 @@ kv_attention_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
         int64_t row;
         if constexpr (PLAIN) row = (int64_t)kvh * p.Sk + pos;
         else row = ((((int64_t)page * p.pages.Hkv + h) << p.pages.page_shift)) + (pos & ((1 << p.pages.page_shift) - 1));
-        if (!there && pos >= 0) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); }
+        if (!there && pos >= 0) { *bad = 1; ptx::report(p.page_status, KV_ERR_PAGE); }
         look_up(j + 1);
         const uint32_t n_there = NG == 1 ? (there ? 1 : 0) : __popc(__ballot_sync(0xffffffffu, there));
         if (lane == 0) ptx::mbar_arrive_expect_tx(full + 8 * slot, n_there * (16 * 2 * ROW));

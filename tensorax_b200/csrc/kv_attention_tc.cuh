@@ -146,7 +146,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
 
     if (tid == 0) {
         *bad = beyond ? 1 : 0;
-        if (beyond) ptx::report(p.status, KV_ERR_PAGE);
+        if (beyond) ptx::report(p.page_status, KV_ERR_PAGE);
         *abort_flag = 0;
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(k_ready + 8 * t, Cfg::CONVERTERS);     // one arrival per converter warp
@@ -272,7 +272,7 @@ kv_attention_tc_kernel(const __grid_constant__ KvAttnParams p)
         auto first_row = [&](int j) -> int {
             const int c = c_from + j * BN + lane * 16, pos = c < s_end ? c : c + skip;
             if (!wanted(j)) return -1;
-            if (page < 0 || page >= p.pages.pages) { *bad = 1; ptx::report(p.status, KV_ERR_PAGE); return -1; }
+            if (page < 0 || page >= p.pages.pages) { *bad = 1; ptx::report(p.page_status, KV_ERR_PAGE); return -1; }
             return ((page * p.pages.Hkv + h) << p.pages.page_shift) + (pos & ((1 << p.pages.page_shift) - 1));
         };
         float kc[4], vc[4];                                       // scales of keys lane, lane + 32, ... of a tile

@@ -10,7 +10,8 @@
 //
 // Pages: k, v [pages, kv_heads, page_size, D] bytes, scales [pages, kv_heads, page_size].  The page table [batch, table_len]
 // says where token `pos` of a sequence lies: entry pos / page_size, place pos % page_size.  An entry outside [0, pages), or
-// a position beyond the table, is never followed: the row is left out and the failure word says KV_ERR_PAGE.
+// a position beyond the table, is never followed: the row is left out and KV_ERR_PAGE reported, in a word of its own, since a
+// report in the word for waits that ran out would stop what is queued behind, and the sequences that are not concerned.
 //
 // Both kernels' bound: HBM.  A lane holds eight elements, so a row is D / 8 lanes side by side and every access is 16
 // (values) or 8 (codes) contiguous bytes a lane; K and V of KV_MOVE_STEPS rows are requested before the first is worked on.  A CTA
@@ -52,7 +53,7 @@ struct KvMoveParams {
     const int32_t *pick;      // write only, optional [batch, tokens]: token t is row pick[b, t] of k and v
     int ctas;                 // CTAs that share a head of a sequence
     int tokens, src_tokens;   // src_tokens: rows a head of k and v has
-    int *status;
+    int *page_status;
 };
 
 // Eight values of a lane as they are in memory, and as floats
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(KV_MOVE_THREADS) kv_write_kernel(const KvMoveP
     }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-        if (wanted[s] && to[s] < 0 && gl == 0) ptx::report(p.status, KV_ERR_PAGE);
+        if (wanted[s] && to[s] < 0 && gl == 0) ptx::report(p.page_status, KV_ERR_PAGE);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
             float x[8];
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(KV_MOVE_THREADS) kv_read_kernel(const KvMovePa
         const int t = item.t0 + s * item.STEP;
         rows[s] = t < item.count ? p.pages.row(item.b, item.h, item.start + t) : -1;
         ok[s] = false;
-        if (t < item.count && rows[s] < 0 && gl == 0) ptx::report(p.status, KV_ERR_PAGE);
+        if (t < item.count && rows[s] < 0 && gl == 0) ptx::report(p.page_status, KV_ERR_PAGE);
     }
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {

@@ -83,7 +83,7 @@ int move_rows(const char *who, const tx_kv_cache &c, const void *k, const void *
     if (!pick && src_tokens < tokens) return fail(TX_ERR_INVALID, "%s: k and v hold fewer rows than tokens", who);
     if (tokens > 0x3fffffffLL || src_tokens > 0x3fffffffLL) return fail(TX_ERR_UNSUPPORTED, "%s: dimension too large", who);
     if (int rc = txb::api::ensure_device()) return rc;
-    if (int rc = txb::api::status_word(&p.status)) return rc;
+    if (int rc = txb::api::page_word(&p.page_status)) return rc;
     p.k = const_cast<void *>(k); p.v = const_cast<void *>(v);
     p.start = start; p.counts = counts; p.pick = pick;
     p.tokens = (int)tokens; p.src_tokens = (int)src_tokens;
@@ -286,6 +286,7 @@ int tx_kv_cache_attention(const tx_kv_attention_desc *d)
     if (d->flags & ~TX_SDPA_OUT_F16) return fail(TX_ERR_INVALID, "%s: unknown flags", who);
     if (int rc = txb::api::ensure_device()) return rc;
     if (int rc = txb::api::status_word(&p.status)) return rc;
+    if (int rc = txb::api::page_word(&p.page_status)) return rc;
     p.q = d->q; p.out = d->out;
     p.kv_lens = d->kv_lens; p.q_lens = d->q_lens; p.tree = d->tree;
     p.tokens = (int)d->tokens; p.group = (int)(d->q_heads / d->cache.kv_heads);

@@ -111,9 +111,14 @@ void pool_free(char *p, cudaStream_t st)
 // One status word per device, written by kernels whose bounded waits run out, and its mirror in pinned host memory
 // (the device address of the mirror sits behind the word, see ptx::report): asking for it after a synchronise is a
 // load, where copying the word back was a second trip to the device on every call (7 us of a 47 us call).
-struct Status {
+// Later launches look at that word and stop.  A page or row that does not exist concerns its own sequence only: it is reported in
+// a second word, which no kernel reads.
+struct Word {
     int *word = nullptr;
     volatile int *mirror = nullptr;
+};
+struct Status {
+    Word waits, pages;
 };
 Status g_status[kMaxDevices];
 std::atomic<bool> g_status_ready[kMaxDevices] = {};
@@ -127,19 +132,33 @@ int status_word(int **out)
         std::lock_guard<std::mutex> lk(g_status_mu);
         if (!g_status_ready[dev].load(std::memory_order_relaxed)) {
             Status s;
-            int *mirror = nullptr, *mirror_dev = nullptr;
-            TX_CUDA(cudaMalloc(&s.word, 256));
+            int *words = nullptr, *mirror = nullptr, *mirror_dev = nullptr;
+            TX_CUDA(cudaMalloc(&words, 256));
             TX_CUDA(cudaHostAlloc(&mirror, 64, cudaHostAllocMapped));
-            *mirror = 0;
-            s.mirror = mirror;
             TX_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void **>(&mirror_dev), mirror, 0));
-            TX_CUDA(cudaMemset(s.word, 0, 256));
-            TX_CUDA(cudaMemcpy(s.word + 2, &mirror_dev, sizeof mirror_dev, cudaMemcpyHostToDevice));
+            TX_CUDA(cudaMemset(words, 0, 256));
+            int n = 0;
+            for (Word *w : {&s.waits, &s.pages}) {              // 128 and 32 bytes apart
+                w->word = words + 32 * n;
+                w->mirror = mirror + 8 * n;
+                *w->mirror = 0;
+                int *at = mirror_dev + 8 * n++;
+                TX_CUDA(cudaMemcpy(w->word + 2, &at, sizeof at, cudaMemcpyHostToDevice));
+            }
             g_status[dev] = s;
             g_status_ready[dev].store(true, std::memory_order_release);
         }
     }
-    *out = g_status[dev].word;
+    *out = g_status[dev].waits.word;
+    return TX_OK;
+}
+
+int page_word(int **out)
+{
+    int dev = 0;
+    if (int rc = status_word(out)) return rc;                   // sets both up
+    if (int rc = current_device(&dev)) return rc;
+    *out = g_status[dev].pages.word;
     return TX_OK;
 }
 
@@ -1099,17 +1118,21 @@ int finish(cudaStream_t st)
     TX_CUDA(cudaStreamSynchronize(st));
     int dev = 0;
     if (int rc = current_device(&dev)) return rc;
-    if (!g_status_ready[dev].load(std::memory_order_acquire) || *g_status[dev].mirror == 0) return TX_OK;
+    if (!g_status_ready[dev].load(std::memory_order_acquire) || (*g_status[dev].waits.mirror == 0 && *g_status[dev].pages.mirror == 0)) return TX_OK;
     std::lock_guard<std::mutex> lk(g_status_mu);
-    const int code = txb::take_report(
-        [&](int v) { return __atomic_exchange_n(const_cast<int *>(g_status[dev].mirror), v, __ATOMIC_SEQ_CST); },
-        // the word only: the mirror's address stays behind it
-        [&] { return cudaMemset(g_status[dev].word, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess; });
-    if (code == txb::KV_ERR_PAGE)
-        return fail(TX_ERR_KERNEL, "K/V cache: a token lies outside its sequence's page table, or the table or the row list names "
-                                   "a page or row that does not exist (stage code %d); output is not valid", code);
+    auto take = [&](const Word &w) {
+        return txb::take_report(
+            [&](int v) { return __atomic_exchange_n(const_cast<int *>(w.mirror), v, __ATOMIC_SEQ_CST); },
+            // the word only: the mirror's address stays behind it
+            [&] { return cudaMemset(w.word, 0, sizeof(int)) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess; });
+    };
+    const int code = take(g_status[dev].waits), page = take(g_status[dev].pages);
     if (code != 0)
-        return fail(TX_ERR_KERNEL, "SDPA kernel gave up on a bounded wait (stage code %d); output is not valid", code);
+        return fail(TX_ERR_KERNEL, "SDPA kernel gave up on a bounded wait (stage code %d); output is not valid%s", code,
+                    page ? "; a K/V cache call named a page or row that does not exist, too" : "");
+    if (page != 0)
+        return fail(TX_ERR_KERNEL, "K/V cache: a token lies outside its sequence's page table, or the table or the row list names "
+                                   "a page or row that does not exist (stage code %d); output is not valid", page);
     return TX_OK;
 }
 
@@ -1506,6 +1529,7 @@ int fail(int code, const char *fmt, ...)
 }
 int ensure_device() { return ::ensure_device(); }
 int status_word(int **out) { return ::status_word(out); }
+int page_word(int **out) { return ::page_word(out); }
 int sm_count(int *n) { return ::sm_count(n); }
 int current_device(int *dev) { return ::current_device(dev); }
 int map_of_codes(CUtensorMap *m, const void *base, int64_t rows, int64_t d) { return make_map(m, base, 1, rows * d / 128, 128, (int)(d / 8), 1); }
@@ -2136,9 +2160,6 @@ int tx_sdpa_fp16_static_scratch(const void *Q_h, const void *K_h, const void *V_
     int code = 0;
     TX_CUDA(cudaMemcpyAsync(&code, status, sizeof code, cudaMemcpyDeviceToHost, st));
     TX_CUDA(cudaStreamSynchronize(st));
-    if (code == txb::KV_ERR_PAGE)
-        return fail(TX_ERR_KERNEL, "K/V cache: a token lies outside its sequence's page table, or the table or the row list names "
-                                   "a page or row that does not exist (stage code %d); output is not valid", code);
     if (code != 0)
         return fail(TX_ERR_KERNEL, "SDPA kernel gave up on a bounded wait (stage code %d); output is not valid", code);
     return TX_OK;
