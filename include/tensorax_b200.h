@@ -317,7 +317,7 @@ TX_API int tx_sdpa_backward(const tx_sdpa_bwd_desc *desc);
  *      valid key within 128 keys of one that some row of a 128-row tile sees may show in all rows of the tile (decoding steps of up
  *      to 16 rows a K/V head: at a key that one of them sees).
  *      Backward: as tx_sdpa_backward (fp16, d in {64, 128, 256}); a row that sees no key has gradient zero and adds nothing to
- *      those of K and V.  TX_BWD_GRADS_F16: dq, dk, dv are fp16. */
+ *      those of K and V, whatever its query and the gradient of its result hold.  TX_BWD_GRADS_F16: dq, dk, dv are fp16. */
 enum { TX_BWD_GRADS_F16 = 64 };
 typedef struct tx_window_desc {
     int64_t window;              /* 1 at least: a row's own position counts */

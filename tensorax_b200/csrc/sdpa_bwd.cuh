@@ -866,6 +866,9 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                        t_dk = tmem + lane_base + Cfg::COL_DK, t_dv = tmem + lane_base + Cfg::COL_DV,
                        t_p = tmem + lane_base + Cfg::COL_P + c0 / 2, t_ds = tmem + lane_base + Cfg::COL_DS + c0 / 2;
         const bool key_ok = key < kv_limit;
+        // window: queries that see no key, in front of `front` and from `behind` on, may hold anything
+        const int front = Cfg::WINDOW ? p.win.front(off) : 0;
+        const int behind = Cfg::WINDOW && max(p.win.sinks, p.apart_k) == 0 ? p.win.behind(kv_limit, off) : 0x7fffffff;
         bool ok = run;
         auto arrive_warp = [&](uint32_t bar) {
             ptx::tc_fence_before_sync();
@@ -966,6 +969,12 @@ sdpa_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
                 ptx::tmem_st_cols<CW / 2>(t_p, pp);
                 ptx::tmem_st_cols<CW / 2>(t_ds, pd);
                 ptx::tmem_wait_st();
+            }
+            if (Cfg::WINDOW && (qr0 < front || qr0 + BQ > behind)) {      // for dS^T Q, where their columns of dS^T are zero
+                uint8_t *q_stage = smem + Cfg::OFF_Q + (t % NS) * Cfg::Q_BYTES;
+                zero_stage_rows<BQ, 128 * Cfg::WGS>(q_stage, Cfg::KP, 0, st, min(max(front - qr0, 0), BQ));
+                zero_stage_rows<BQ, 128 * Cfg::WGS>(q_stage, Cfg::KP, min(max(behind - qr0, 0), BQ), st);
+                ptx::fence_proxy_async_smem();
             }
             arrive_warp(pds_full);
         }

@@ -75,7 +75,7 @@ sdpa_bwd_sinks_kernel(const __grid_constant__ SinkGradParams p)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = lane >> 2, t4 = lane & 3;
 
     const int kvh = (int)blockIdx.x / splits, last = min(p.win.sinks, p.Sk);           // batch element and K/V head
-    const int limit = p.kv_lens.limit(kvh / p.Hkv, p.Sk), off = p.win.offset(limit, p.Sq);
+    const int limit = p.kv_lens.limit(kvh / p.Hkv, p.Sk), off = p.win.offset(limit, p.Sq), front = p.win.front(off);
     const int64_t rows = (int64_t)p.group * p.Sq, first_row = (int64_t)kvh * rows;    // a head's rows follow the one before's
     const int steps = limit > 0 ? (int)((rows + 15) / 16) : 0;
 
@@ -101,14 +101,19 @@ sdpa_bwd_sinks_kernel(const __grid_constant__ SinkGradParams p)
     auto request = [&](int j) {
         const uint32_t stage = ring + j % NS * Cfg::STAGE;
         const int64_t row0 = ((int64_t)rank + (int64_t)j * every) * 16;
+        auto copy = [&](auto there) {
 #pragma unroll 4
-        for (int i = lane; i < 2 * 16 * CHUNKS; i += 32) {
-            const int r = i / CHUNKS % 16, c = i % CHUNKS;
-            const __half *src = i < 16 * CHUNKS ? p.q : p.dout;
-            const uint32_t dst = stage + (i < 16 * CHUNKS ? 0 : Cfg::TILE) + at(r, c);
-            if (row0 + r < rows) ptx::cp_async16(sbase + dst, src + (first_row + row0 + r) * D + c * 8);
-            else *reinterpret_cast<uint4 *>(smem + dst) = make_uint4(0u, 0u, 0u, 0u);
-        }
+            for (int i = lane; i < 2 * 16 * CHUNKS; i += 32) {
+                const int r = i / CHUNKS % 16, c = i % CHUNKS;
+                const __half *src = i < 16 * CHUNKS ? p.q : p.dout;
+                const uint32_t dst = stage + (i < 16 * CHUNKS ? 0 : Cfg::TILE) + at(r, c);
+                if (there(r)) ptx::cp_async16(sbase + dst, src + (first_row + row0 + r) * D + c * 8);
+                else *reinterpret_cast<uint4 *>(smem + dst) = make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        // queries in front of the first key see none and may hold anything: zero
+        if (front > 0) copy([&](int r) { return row0 + r < rows && (int)((row0 + r) % p.Sq) >= front; });
+        else copy([&](int r) { return row0 + r < rows; });
         if (row0 + (lane & 15) < rows)
             ptx::cp_async4(sbase + stage + 2 * Cfg::TILE + lane * 4, (lane < 16 ? p.lse : p.delta) + first_row + row0 + (lane & 15));
     };

@@ -13,6 +13,10 @@ struct WindowRule {
     int window = 0, sinks = 0, align_end = 0;
     // Position of row 0 of a batch element with `limit` keys
     __device__ __forceinline__ int offset(int limit, int Sq) const { return align_end ? limit - Sq : 0; }
+    // Of a batch element with keys, the rows that see none: those in front of row `front`, and without sinks those from row
+    // `behind` on
+    __device__ __forceinline__ int front(int off) const { return max(0, -off); }
+    __device__ __forceinline__ int behind(int limit, int off) const { return (int)min((int64_t)0x7fffffff, (int64_t)limit + window - 1 - off); }
 };
 
 // The key tiles of BN keys that rows at positions [pos0, pos0 + rows) walk: list entry j is tile j for j < n_sink, else
@@ -76,13 +80,13 @@ __device__ __forceinline__ float zero_unless_within(float v, int i, int lo, int 
     return r;
 }
 
-// Rows [from, BN) of a stage of `panels` panels [BN][128 bytes] become zero: keys behind a sequence's last, whatever they
-// hold (a zero weight times a NaN would be one).  THREADS threads share them; the caller orders the writes before the MMA
-// that reads the stage.
+// Rows [from, to) of a stage of `panels` panels [BN][128 bytes] become zero: keys behind a sequence's last, queries that see no
+// key, whatever they hold (a zero weight times a NaN would be one).  THREADS threads share them; the caller orders the writes
+// before the MMA that reads the stage.
 template <int BN, int THREADS>
-__device__ __forceinline__ void zero_stage_rows(uint8_t *stage, int panels, int from, int thread)
+__device__ __forceinline__ void zero_stage_rows(uint8_t *stage, int panels, int from, int thread, int to = BN)
 {
-    const int chunks = (BN - from) * 8;
+    const int chunks = (to - from) * 8;
     for (int pn = 0; pn < panels; ++pn)
         for (int i = thread; i < chunks; i += THREADS)
             *reinterpret_cast<uint4 *>(stage + pn * (BN * 128) + from * 128 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
