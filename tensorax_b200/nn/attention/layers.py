@@ -56,6 +56,8 @@ class GroupedQueryAttention:
             if mask is not None:
                 raise ValueError("forward_bhsd: a window takes no dense mask")
             return F.scaled_dot_product_attention_window(query, key, value, window, sinks, kv_lens=kv_lens, align=align)
+        if sinks or align != "start":
+            raise ValueError("forward_bhsd: sinks and align belong to a window")
         return F.scaled_dot_product_attention_ex(query, key, value, mask, causal=causal, kv_lens=kv_lens)
 
     def forward_cached(self, query: Tensor, cache, page_table, kv_lens, q_lens=None, tree=None, window=None,
