@@ -170,7 +170,9 @@ __device__ __forceinline__ void store_grad_half(const uint8_t *tile, __half *dst
 // at d = 64, 32 otherwise, four values a lane and step; a warp requests two steps of rows at a time.  One row a warp and
 // eight bytes a lane took 30.3 us at B4 H16 S2048 d128, this 23.4 (6.9 TB/s; dO and O partly in L2).
 // With a window a row that sees no key gets dO and delta zero, whatever the caller's gradient of its NaN is: in the products that
-// add up dK and dV its weight of zero would not keep a NaN out.
+// add up dK and dV its weight of zero would not keep a NaN out.  And delta is that of dO as rounded, which is what dO V^T is
+// formed of: dS is the difference of the two, and small where few keys are seen (one key: nothing).  With delta of dO in fp32
+// dQ and dK were 8e-4 of their norm off in a padded batch whose last rows see a few keys each, with this 4e-4.
 struct PrepWindow {
     KvLens kv_lens;
     WindowRule rule;
@@ -225,10 +227,17 @@ __global__ void __launch_bounds__(256) sdpa_bwd_prep_kernel(const float *__restr
                 for (int c = 0; c < PIECES; ++c) g[t][c] = o[t][c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < PIECES; ++c) {
-            const float4 a = g[t][c], b = o[t][c];
+            float4 a = g[t][c];
+            const float4 b = o[t][c];
+            const __half2 lo = __floats2half2_rn(a.x, a.y), hi = __floats2half2_rn(a.z, a.w);
+            if constexpr (WINDOW) {
+                const float2 l = __half22float2(lo), h = __half22float2(hi);
+                a = make_float4(l.x, l.y, h.x, h.y);
+            }
             acc = fmaf(a.x, b.x, acc); acc = fmaf(a.y, b.y, acc); acc = fmaf(a.z, b.z, acc); acc = fmaf(a.w, b.w, acc);
             if (row < rows)
-                *reinterpret_cast<uint2 *>(dout_h + row * D + (c * LPR + gl) * 4) = make_uint2(ptx::pack_half2(a.x, a.y), ptx::pack_half2(a.z, a.w));
+                *reinterpret_cast<uint2 *>(dout_h + row * D + (c * LPR + gl) * 4) =
+                    make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
         }
 #pragma unroll
         for (int w = LPR / 2; w > 0; w >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, w);
