@@ -27,9 +27,9 @@
 // fp32 queries: Q (scaled by a power of two per row) and P are carried as two fp16 numbers each, and the products of a
 // stage are added to O in fp32 instead of in the matrix unit, whose sums are cut off rather than rounded.
 //
-// The same kernel takes decoding steps of the windowed attention over plain fp16 keys (KV_PLAIN), weights as two numbers each as
-// everywhere in decoding steps: B8 Hq32 Hkv8 d128, window 2048, four sinks, 16.9 us, 27.7 by the kernel of sdpa_decode.cuh, whose
-// products are fp32 FMAs.
+// The same kernel takes decoding steps of the windowed attention over plain fp16 keys (KV_PLAIN): B8 Hq32 Hkv8 d128, window 2048,
+// four sinks, 16.9 us, 27.7 by the kernel of sdpa_decode.cuh, whose products are fp32 FMAs.  Weights are two numbers each there, as
+// that kernel's are fp32; over the cache fp16 queries have one (2^-11, below the codes' own rounding of 2^-4 or 1/254).
 #pragma once
 #include <cfloat>
 #include <cooperative_groups.h>

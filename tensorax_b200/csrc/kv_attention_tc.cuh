@@ -3,7 +3,7 @@
 //
 // Bound: the tensor pipe and the softmax's exponentials, as in sdpa_tc_pair_kernel, whose softmax, issue order and tensor-memory
 // layout (P over S) this kernel has.  mma.sync, which the other kernel uses, does a third of tcgen05's work at best (549 TFLOP/s
-// measured); at 256 rows a head it took 341 us where this kernel takes 95 us (B8 Hkv8, 8192 keys in the window, d 128: 724 TFLOP/s).
+// measured); at 256 rows a head it took 341 us where this kernel takes 96 us (B8 Hkv8, 8192 keys in the window, d 128: 717 TFLOP/s).
 //
 // One CTA: two 128-row query tiles of one (batch, K/V head) and a share of the keys in tiles of 128; CTAs of a cluster share the
 // keys and add their results in rank order.
@@ -17,7 +17,8 @@
 // largest ks of the tile and vref the same of vs over the tiles so far.  Both quotients are at most 1, kref joins the softmax
 // scale, and O is rescaled when vref grows.  e4m3 scales are powers of two: the products are exact down to fp16's smallest
 // numbers, 2^-24 against 224 in the tile's largest row; int8 products are rounded to fp16 once (2^-11), as a cache in fp16 is.
-// A row whose scale is not finite gets NaN keys and zero values: only the rows that see it are touched.
+// A row whose scale is not finite gets NaN keys and zero values: only the rows that see it are touched, by their maximum, which
+// keeps a NaN that the polynomial exponential would drop, and their sum.
 // Every mbarrier wait is bounded.
 #pragma once
 #include "kv_attention.cuh"

@@ -186,7 +186,8 @@ int launch_attention_tc(txb::KvAttnParams p, const tx_kv_attention_desc *d)
 // More query rows per K/V head than this: the tcgen05 kernel, whose CTA takes 256 at once.  Hkv8, us there and here, e4m3:
 // B8, 8192 keys, d128: 32 rows 81 and 50, 64 rows 82 and 86; d64: 65 and 35, 65 and 63; B1, 2000 keys, d128: 18 and 16, 19 and 26;
 // B16, 1000 keys: 28 and 24, 29 and 31.  int8, whose codes take longer to turn into fp16: 64 rows 105 and 94, 73 and 65, 20 and 26,
-// 35 and 33.  128 rows, e4m3, B8: 83 and 162.
+// 35 and 33.  128 rows, e4m3, B8: 83 and 162.  d256 and fp32 queries have the other kernel only, whose parts of up to 16 or 32
+// rows read and convert the keys each for itself.
 template <int FMT>
 constexpr int kTcRows = FMT == txb::KV_E4M3 ? 32 : 64;
 

@@ -48,7 +48,8 @@ enum PairSection : int {
 };
 
 // POLY: bit e set = element e of every group of 16 exponentials is evaluated on the FMA pipe
-//       (bits come in pairs 2k, 2k+1: the polynomial works on two-wide fp32 vectors).
+//       (bits come in pairs 2k, 2k+1: the polynomial works on two-wide fp32 vectors).  A NaN is lost there: the row's maximum
+//       keeps it (B4 H8 S8192 d64 641 us without that and 639 with, d128 860 and 865).
 // FAULT_TEST: the instantiation behind tx_selftest_wait_timeout -- every wait gives up after 2 ms instead of 2 s and
 //       the producer leaves out the K tile TcParams::skip_k_tile names, so that the give-up path can be exercised
 //       on a GPU without faulting or hanging anything.

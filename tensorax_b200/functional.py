@@ -217,7 +217,8 @@ def kv_cache_attention(query: Tensor, cache, page_table, kv_lens, q_lens=None, t
     """Attention of each sequence's last tokens over the cache they have been written to: one decoding step (T = 1), a chain, or
     with ``tree`` a tree of drafted tokens.  ``query`` [B, heads, T, d] with T <= 64; ``kv_lens[b]`` keys of sequence b, of
     which the last ``q_lens[b]`` (T) are this call's nodes; bit u of ``tree[b][t]`` says that node t sees node u (itself
-    included).  ``window``: a node sees only that many positions up to its own, and the first ``sinks`` keys.  No gradient."""
+    included).  ``window``: a node sees only that many positions up to its own, and the first ``sinks`` keys (None, or 0: all
+    of them).  A page that does not exist is an error, and makes NaN of its own sequence's rows alone.  No gradient."""
     _check_cache(cache, query)
     if query.requires_grad:
         raise ValueError("K/V cache: attention over a cache has no backward pass")
